@@ -12,8 +12,10 @@ from typing import Optional
 
 import torch
 
+from .block_scaled import BlockScaled, block_linear, block_scaled, quantize_blocks
 from .library import (KernelError, call, check, declare, dtype_code, launch_count, library, pointer,
                       require_device, stream_handle, wait_error_flag)
+from .logit_controls import LogitControls, bias_lists, control_logits, sample_controlled, token_masks
 from .stream import STREAM_MANY_ROWS, STREAM_ROWS, RowScaled, StreamSink, stream_rows
 
 __all__ = ["KernelError", "embedding", "add_rmsnorm", "rmsnorm", "silu_mul", "sample", "qk_norm_rope_kv_write",
@@ -23,7 +25,8 @@ __all__ = ["KernelError", "embedding", "add_rmsnorm", "rmsnorm", "silu_mul", "sa
            "RowScaled", "StreamSink", "STREAM_ROWS", "STREAM_MANY_ROWS", "stream_rows", "unscaled_rows_supported", "norm_rope_units", "rotate_units", "attention_diff", "gla_supported",
            "gla_recurrent", "head_linear", "relu_squared", "tanh_narrow", "softcap_", "scaled_sum", "token_shift_mix",
            "short_conv_units", "matrix_recurrence_supported", "wkv_recurrent", "delta_rule_recurrent", "retention_recurrent", "ssd_recurrent", "decay_recurrence_supported",
-           "gelu_mul", "grouped_rmsnorm", "conv_norm_kv", "streams_norm", "unit_linear_wide", "gated_scan"]
+           "gelu_mul", "grouped_rmsnorm", "conv_norm_kv", "streams_norm", "unit_linear_wide", "gated_scan", "BlockScaled", "block_scaled", "quantize_blocks",
+           "LogitControls", "control_logits", "bias_lists", "token_masks"]
 
 
 def embedding(table: torch.Tensor, ids: torch.Tensor, out: Optional[torch.Tensor] = None, scale: float = 1.0,
@@ -164,10 +167,15 @@ def clamped_gate_up(x: torch.Tensor, weight: torch.Tensor, limit: float, alpha: 
 
 
 def sample(logits: torch.Tensor, temperatures: Optional[torch.Tensor] = None, seeds: Optional[torch.Tensor] = None,
-           steps: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, flags=None) -> torch.Tensor:
+           steps: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, flags=None,
+           controls: Optional[LogitControls] = None, note: bool = False) -> torch.Tensor:
     """One token per row of float32 logits [R, V]: argmax where the temperature is 0, else the
     Gumbel-max draw keyed by (seeds[r], steps[r]).  Returns int32 [R].  ``flags``: two one-element int32 tensors whose
-    values follow the tokens; the result is then [R + 2]."""
+    values follow the tokens; the result is then [R + 2].
+
+    ``controls``: the tokens are drawn from ``control_logits(logits, controls)``, which is not written; a row whose controls leave
+    nothing to draw from gets -1.  ``note``: each token drawn is written behind its request's history (history[history_rows[r],
+    lengths[r]], where there is room), after all rows' histories have been read."""
     check(logits, "logits", torch.float32)
     rows, vocab = logits.shape
     if temperatures is not None:
@@ -184,6 +192,10 @@ def sample(logits: torch.Tensor, temperatures: Optional[torch.Tensor] = None, se
             check(flag, "flag", torch.int32, 1)
         if out.numel() != rows + 2 or rows == 0:
             raise KernelError(f"{rows} tokens and two flags do not fit {out.numel()} elements")
+    if controls is not None:
+        return sample_controlled(logits, temperatures, seeds, steps, out, flags, controls, note)
+    if note:
+        raise KernelError("tokens are noted in the history of controls, and none were given")
     slices = library().llm_sample_slices(rows, vocab)
     scores = indices = None
     if slices > 1:      # large vocabularies are scanned by several blocks per row, merged by a second kernel
@@ -1368,9 +1380,13 @@ def linear(x, weight: torch.Tensor, out: Optional[torch.Tensor] = None,
     PyTorch) where the reference's engine uses a library too, or this package's own kernels where
     they apply (see ``gemm_bf16``).  ``x`` may be a ``RowScaled``.  With a ``sink`` the product is added to the sink's
     residual stream by the product kernel itself where that kernel takes the case (``sink.added`` then says so and
-    nothing is returned); otherwise the sink is left alone and the product is returned as usual."""
+    nothing is returned); otherwise the sink is left alone and the product is returned as usual.
+
+    A ``BlockScaled`` weight (8 bits, a scale for each 128 x 128): see ``block_linear``; ``x`` may then be a ``BlockScaled`` of rows."""
     if x.device.type != "cuda":
         raise KernelError("linear: there is no CPU path")
+    if isinstance(weight, BlockScaled):
+        return block_linear(x, weight, out=out, out_dtype=out_dtype)
     if x.dtype == torch.float32:
         result = gemm_f32(x, weight, out, settled=True)
         return result

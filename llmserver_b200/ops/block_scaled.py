@@ -1,0 +1,158 @@
+"""Rows and matrices in 8 bits (e4m3) with a 32-bit scale for each block, and products of them.
+
+A ``BlockScaled`` of ``block_rows`` 128 is a projection's matrix W [out, in] as checkpoints in 8 bits keep it: a scale for each
+128 x 128.  One of ``block_rows`` 1 holds rows of activations: a scale for each row and 128 columns.  ``ops.linear`` takes the first
+in place of a weight, and either a plain tensor (brought to 8 bits on the way) or the second as its rows:
+
+    weight = ops.quantize_blocks(w, 128)                       # once, when the weights are loaded
+    y = ops.linear(x, weight)                                  # x bfloat16 or float32 [N, in]
+    rows = ops.quantize_blocks(x)                              # once for several products of the same rows
+    a, b = ops.linear(rows, weight_a), ops.linear(rows, weight_b)
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from .library import KernelError, call, check, current_device, dtype_code, stream_handle, wait_error_flag
+
+BLOCK = 128
+FLOAT8 = torch.float8_e4m3fn
+
+
+def _blocks(count: int, size: int = BLOCK) -> int:
+    return -(-count // size)
+
+
+def _pitch(inner: int) -> int:
+    """Bytes from one row to the next: the copies of the product kernel begin at multiples of 16 bytes."""
+    return -(-inner // 16) * 16
+
+
+@dataclass
+class BlockScaled:
+    """``values`` (float8_e4m3fn [rows, columns]) times ``scales`` (float32 [ceil(rows / block_rows), ceil(columns / 128)]), each scale for
+    ``block_rows`` (1 or 128) rows and 128 columns.  The rows of ``values`` may lie apart (``values.stride(0)``); the product kernel wants
+    them at multiples of 16 bytes, which ``block_scaled`` sees to."""
+    values: torch.Tensor
+    scales: torch.Tensor
+    block_rows: int = BLOCK
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.values.dtype
+
+    def widened(self) -> torch.Tensor:
+        """The numbers that this stands for, float32."""
+        rows, columns = self.values.shape
+        wide = self.scales.repeat_interleave(BLOCK, dim=1)[:, :columns]
+        return self.values.float() * (wide if self.block_rows == 1 else wide.repeat_interleave(self.block_rows, dim=0)[:rows])
+
+
+def block_scaled(values: torch.Tensor, scales: torch.Tensor, block_rows: int = BLOCK) -> BlockScaled:
+    """A ``BlockScaled`` of a checkpoint's tensors; ``values`` are copied into rows at multiples of 16 bytes where theirs are not, ``scales``
+    are widened to float32."""
+    result = BlockScaled(values, scales.float().contiguous(), block_rows)
+    if values.dim() == 2 and values.dtype == FLOAT8 and values.shape[1] > 0 and (
+            values.stride(1) != 1 or values.stride(0) % 16 or values.stride(0) < values.shape[1] or values.data_ptr() % 16):
+        rows, columns = values.shape
+        kept = torch.empty((rows, _pitch(columns)), dtype=FLOAT8, device=values.device)[:, :columns]
+        kept.view(torch.uint8).copy_(values.view(torch.uint8))
+        result.values = kept
+    return _checked(result, block_rows, "block-scaled tensor")
+
+
+def _checked(operand: BlockScaled, block_rows: int, name: str) -> BlockScaled:
+    values, scales = operand.values, operand.scales
+    if not (values.is_cuda and scales.is_cuda):
+        raise KernelError(f"{name} must live on a CUDA device (there is no CPU path); it is on {values.device} and {scales.device}")
+    if values.dtype != FLOAT8 or scales.dtype != torch.float32 or values.dim() != 2:
+        raise KernelError(f"{name} must be float8_e4m3fn [rows, columns] with float32 scales, got {values.dtype} {tuple(values.shape)} and {scales.dtype}")
+    if operand.block_rows != block_rows:
+        raise KernelError(f"{name}: scales for {block_rows} rows are needed, these are for {operand.block_rows}")
+    rows, columns = values.shape
+    if columns < 1 or (block_rows > 1 and rows < 1):
+        raise KernelError(f"{name} is empty: {tuple(values.shape)}")
+    if tuple(scales.shape) != (_blocks(rows, block_rows), _blocks(columns)) or not scales.is_contiguous():
+        raise KernelError(f"{name}: {tuple(values.shape)} in blocks of {block_rows} x {BLOCK} has contiguous scales "
+                          f"[{_blocks(rows, block_rows)}, {_blocks(columns)}], got {tuple(scales.shape)} with strides {scales.stride()}")
+    stride = values.stride(0) if rows > 1 else max(values.stride(0), _pitch(columns))
+    if (values.stride(1) != 1 and columns > 1) or stride % 16 or stride < columns or values.data_ptr() % 16:
+        raise KernelError(f"{name}: rows must begin at multiples of 16 bytes (strides {values.stride()}, address {values.data_ptr():#x}); "
+                          "block_scaled() copies them so")
+    return operand
+
+
+def _row_stride(values: torch.Tensor) -> int:
+    """Bytes between rows; of a single row whatever the kernel may be told."""
+    return values.stride(0) if values.shape[0] > 1 else _pitch(values.shape[1])
+
+
+def quantize_blocks(x: torch.Tensor, block_rows: int = 1) -> BlockScaled:
+    """``x`` (float32 or bfloat16 [rows, columns]) in 8 bits: with ``block_rows`` 1 a scale for each row and 128 columns, with 128 one for
+    each 128 x 128.  A scale is 2^e with the least e (not below -126) for which no number of the block exceeds 448 * 2^e; the numbers
+    are divided by it and rounded to the nearest of e4m3's, ties to the even one.  A block that holds an infinity or a NaN becomes NaN."""
+    check(x, "x")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise KernelError(f"quantize_blocks takes a matrix, got {tuple(x.shape)}")
+    if block_rows not in (1, BLOCK):
+        raise KernelError(f"blocks have 1 or {BLOCK} rows, not {block_rows}")
+    current_device(x, "x")
+    rows, columns = x.shape
+    pitch = _pitch(columns)
+    values = torch.empty((rows, pitch), dtype=FLOAT8, device=x.device)
+    scales = torch.empty((_blocks(rows, block_rows), _blocks(columns)), dtype=torch.float32, device=x.device)
+    call("llm_quantize_blocks", x.data_ptr(), dtype_code(x.dtype), values.data_ptr(), scales.data_ptr(), rows, columns, pitch, int(block_rows),
+         stream_handle())
+    return BlockScaled(values if pitch == columns else values[:, :columns], scales, block_rows)
+
+
+def block_linear(x, weight: BlockScaled, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y = x W^T for W in 8 bits: what ``ops.linear`` does with a ``BlockScaled`` weight.  ``x`` [N, in]: float32 or bfloat16 (brought to 8
+    bits as ``quantize_blocks`` does), or a ``BlockScaled`` of single rows.  Sums and scales are 32-bit; the result is rounded once to
+    ``out_dtype`` (float32 or bfloat16; default: that of ``out``, or x's, or bfloat16 where x is in 8 bits)."""
+    _checked(weight, BLOCK, "weight")
+    cols, inner = weight.values.shape
+    quantized = isinstance(x, BlockScaled)
+    if quantized:
+        _checked(x, 1, "x")
+    else:
+        check(x, "x")
+        if x.dim() != 2:
+            raise KernelError(f"block_linear takes rows [N, {inner}], got {tuple(x.shape)}")
+    rows = x.shape[0]
+    if x.shape[1] != inner:
+        raise KernelError(f"x has {x.shape[1]} columns, the weight {inner}")
+    device = weight.values.device
+    if x.device != device or (out is not None and out.device != device) or weight.scales.device != device or (quantized and x.scales.device != device):
+        raise KernelError(f"the operands lie on {x.device} and {device}")
+    current_device(weight.values, "weight")
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else torch.bfloat16 if quantized else x.dtype
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"block_linear writes float32 or bfloat16, not {out_dtype}")
+    if out is None:
+        out = torch.empty((rows, cols), dtype=out_dtype, device=device)
+    elif out.dtype != out_dtype or not out.is_contiguous() or tuple(out.shape) != (rows, cols):
+        raise KernelError(f"block_linear: the output must be contiguous {out_dtype} [{rows}, {cols}], got {out.dtype} {tuple(out.shape)}")
+    if quantized:
+        source, kind, values, pitch, scales = 0, 0, x.values.data_ptr(), _row_stride(x.values), x.scales.data_ptr()
+    else:
+        # one piece of scratch: the rows' 8-bit numbers, then their scales
+        pitch = _pitch(inner)
+        scratch = torch.empty(rows * (pitch + 4 * _blocks(inner)), dtype=torch.uint8, device=device)
+        source, kind, values = x.data_ptr(), dtype_code(x.dtype), scratch.data_ptr()
+        scales = values + rows * pitch
+    call("llm_block_linear", source, kind, values, pitch, scales, weight.values.data_ptr(), _row_stride(weight.values), weight.scales.data_ptr(),
+         out.data_ptr(), int(out_dtype == torch.float32), rows, cols, inner, wait_error_flag(device).data_ptr(), stream_handle())
+    return out

@@ -28,6 +28,11 @@ SIGNATURES = {
     "llm_ssd_recurrent": [_P, _I, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _S],
     "llm_sample": [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _S],
     "llm_sample_slices": [_I, _I],
+    "llm_control_slices": [_I, _I],
+    "llm_control_logits": [_P, _P, _I, _I, _P, _S],
+    "llm_control_sample": [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _S],
+    "llm_quantize_blocks": [_P, _I, _P, _P, _I, _I, ctypes.c_longlong, _I, _S],
+    "llm_block_linear": [_P, _I, _P, ctypes.c_longlong, _P, _P, ctypes.c_longlong, _P, _P, _I, _I, _I, _I, _P, _S],
     "llm_qk_norm_rope_kv_write": [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _I, _I, _I, _S],
     "llm_attention_generic": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _I, _S],
     "llm_rope_kv_write_split": [_P, _P, _F, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I, _I, _S],
@@ -193,6 +198,12 @@ def check(tensor: torch.Tensor, name: str, dtype=None, last_dim=None) -> torch.T
     return tensor
 
 
+def current_device(tensor: torch.Tensor, name: str) -> None:
+    """Raises unless the tensor lies on the current device, whose stream a launch goes to."""
+    if tensor.device.index != _device_index():
+        raise KernelError(f"{name} lies on {tensor.device}, the current device is cuda:{_device_index()}")
+
+
 _wait_error_flags = {}
 
 
@@ -215,4 +226,5 @@ def check_wait_errors() -> None:
             raise KernelError(f"a kernel gave up waiting on one of its barriers (code {code}: 2 matrix product, "
                               "3 decode attention, 4 prompt attention), or attention met a block-table entry that names no "
                               "page of the pool (5) or a context that needs more splits than it was given (6), or the experts' "
-                              "tiled product gave up waiting (7); the step's result is invalid")
+                              "tiled product gave up waiting (7), or a row of logits named a history, a bias list or a mask that does "
+                              "not exist (8); the step's result is invalid")
