@@ -8,39 +8,14 @@
 //
 // What bounds it: reading x and writing a byte for each number.  Rows: a warp takes groups of 128 one after the other, four numbers a
 // lane.  Matrices: a block of threads keeps the 128 x 128 numbers in registers between the maximum and the rounding.
-#include "common.cuh"
+#include "block_scaled.cuh"
 
 namespace {
 
-constexpr int kGroup = 128;
+using namespace block_scaled;
+
+constexpr int kGroup = kBlock;
 constexpr int kThreads = 256;
-constexpr uint32_t kInfinity = 0x7f800000u;
-
-// Bits of the 32-bit scale of a block whose largest magnitude has these bits: the exponent field of the magnitude, one more where the mantissa is
-// above 448's (0x600000), less 8.  The caller looks for infinities and NaN.
-__device__ __forceinline__ uint32_t scale_bits(uint32_t largest) { return max((int)((largest + 0x1fffffu) >> 23) - 8, 1) << 23; }
-
-struct Rounding {
-    float scale, inverse;
-};
-__device__ __forceinline__ Rounding rounding_of(uint32_t largest) {
-    const bool finite = largest < kInfinity;
-    const uint32_t bits = finite ? scale_bits(largest) : 0x7fffffffu;
-    Rounding r;
-    r.scale = __uint_as_float(bits);
-    r.inverse = __uint_as_float(finite ? (254u << 23) - bits : 0x7fffffffu);
-    return r;
-}
-
-// Four numbers as e4m3, the first in the lowest byte.
-__device__ __forceinline__ uint32_t four_of(const float (&v)[4], float inverse) {
-    uint16_t low, high;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(low) : "f"(v[1] * inverse), "f"(v[0] * inverse));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(high) : "f"(v[3] * inverse), "f"(v[2] * inverse));
-    return (uint32_t)low | (uint32_t)high << 16;
-}
-
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }      // NaN above infinity above all others
 
 __device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
@@ -81,7 +56,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
         load4(x + (size_t)row * inner, first, inner, whole != 0, v);
         const uint32_t largest = warp_max_bits(max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3]))));
         const Rounding r = rounding_of(largest);
-        if (first < inner) *reinterpret_cast<uint32_t*>(out + (size_t)row * pitch + first) = four_of(v, r.inverse);
+        if (first < inner) *reinterpret_cast<uint32_t*>(out + (size_t)row * pitch + first) = four_of(v[0], v[1], v[2], v[3], r.inverse);
         if (lane == 0) scales[g] = r.scale;
     }
 }
@@ -118,7 +93,7 @@ __global__ void __launch_bounds__(kThreads) quantize_matrix_kernel(const T* __re
     if (first < inner)
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
-            if (row0 + i < rows) *reinterpret_cast<uint32_t*>(out + (size_t)(row0 + i) * pitch + first) = four_of(v[i], r.inverse);
+            if (row0 + i < rows) *reinterpret_cast<uint32_t*>(out + (size_t)(row0 + i) * pitch + first) = four_of(v[i][0], v[i][1], v[i][2], v[i][3], r.inverse);
     if (threadIdx.x == 0) scales[(size_t)blockIdx.y * groups + blockIdx.x] = r.scale;
 }
 
@@ -133,21 +108,20 @@ LLM_EXPORT int llm_quantize_blocks(const void* x, int dtype, void* out, float* s
         return LLM_REFUSED;
     }
     if (rows == 0) return LLM_OK;
-    const int groups = (inner + kGroup - 1) / kGroup;
+    const int groups = (inner + kGroup - 1) / kGroup, row_blocks = (rows + kGroup - 1) / kGroup;
+    if (block_rows != 1 && row_blocks > 65535) {
+        llm_set_error("quantize_blocks: at most %d rows, got %d", 65535 * kGroup, rows);
+        return LLM_REFUSED;
+    }
     LLM_DISPATCH_DTYPE(dtype, {
         // four numbers of every row can be read at once: the rows begin at multiples of four numbers
         const int whole = inner % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
         if (block_rows == 1) {
             const long long warps = (long long)rows * groups, blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
-            const long long most = 8LL * llm_sm_count();      // what runs at a time
-            llm_launch(quantize_rows_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), kThreads, 0, stream,
+            const long long room = 8LL * llm_sm_count();      // blocks that run at a time
+            llm_launch(quantize_rows_kernel<T>, dim3((unsigned)(blocks < room ? blocks : room)), kThreads, 0, stream,
                        reinterpret_cast<const T*>(x), reinterpret_cast<unsigned char*>(out), scales, rows, inner, groups, pitch, whole);
         } else {
-            const int row_blocks = (rows + kGroup - 1) / kGroup;
-            if (row_blocks > 65535) {
-                llm_set_error("quantize_blocks: at most %d rows, got %d", 65535 * kGroup, rows);
-                return LLM_REFUSED;
-            }
             llm_launch(quantize_matrix_kernel<T>, dim3(groups, row_blocks), kThreads, 0, stream, reinterpret_cast<const T*>(x),
                        reinterpret_cast<unsigned char*>(out), scales, rows, inner, groups, pitch, whole);
         }

@@ -8,27 +8,30 @@
 // The roles of the operands are swapped for the hardware, as in gemm_tcgen05.cu: 128 rows of W are the MMA's M, the tokens (16 to
 // 128) its N, so that a product of few tokens streams W and wastes nothing on rows that do not exist.  A stage of the ring is one
 // block of 128 along k: 16 KiB of W and up to 16 KiB of x, which are one swizzle atom wide.  The MMAs of a block go to one of several
-// buffers of tensor memory, so that they run ahead of the four warps that scale and add.  Where tiles are too few for the SMs, k is
-// split over a cluster and the parts are added through distributed shared memory in the order of k.
+// buffers of tensor memory, so that they run ahead of the warps that scale and add.
 //
-// Roles: warp 0 copies (TMA), warp 1 issues the MMAs, warp 2 brings the tokens' scales (asynchronous copies of 4 bytes, several
-// blocks ahead), warp 3 holds the tensor memory, warps 4 to 7 scale and add, a row of W per thread.  All waits are bounded: one that runs out
-// sets error code 2, every role leaves its loop, and the block still frees its tensor memory and meets its cluster.
+// Where tiles do not come out even on the SMs, k is split over a cluster and the parts are added through distributed shared memory in
+// the order of k (see split_of).
+//
+// Roles: warp 0 copies (TMA), warp 1 issues the MMAs, warp 2 leaves each unit's scales (a token's times W's) in shared
+// memory, warp 3 holds the tensor memory, and the other four or eight scale and add, a row of W and up to 64 tokens per thread.  All waits are
+// bounded: one that runs out sets error code 2, every role leaves its loop, and the block still frees its tensor memory and meets its
+// cluster.
 //
 // k need not be a multiple of 128 nor n of 128 nor m of anything: what lies outside is read as zeros (TMA) and not written.
-#include "common.cuh"
+#include "block_scaled.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
 
 namespace {
 
 constexpr int kRows = 128;            // rows of W per tile (UMMA M)
-constexpr int kBlock = 128;           // of k: one stage, one pair of scales
-constexpr int kThreads = 256;
+using block_scaled::kBlock;           // of k: one stage of the ring, one pair of scales
 constexpr int kMaxStages = 12;
-constexpr int kScaleSlots = 8;        // blocks whose token scales are on their way or waiting
-constexpr int kMaxBuffers = 8;
 constexpr int kMaxSplit = 8;
+constexpr int kScaleSlots = 8;        // units whose scales wait to be used
+constexpr int kScalesAhead = 4;       // and those on their way from memory
+constexpr int kMaxBuffers = 8;
 constexpr uint32_t kWBytes = kRows * kBlock;
 
 struct BlockParams {
@@ -42,6 +45,16 @@ struct BlockParams {
     int* error_flag;
 };
 
+// A place in a ring and the parity of its turn.  It moves by additions: a division of integers is a hundred cycles for a role that one warp
+// plays, and with five of them per unit a unit took 1150 cycles, whatever its size.
+struct Turn {
+    int at = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void step(int size) {
+        if (++at == size) at = 0, parity ^= 1;
+    }
+};
+
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
@@ -51,23 +64,39 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a, uint64_t b, 
 // e4m3 x e4m3 -> float32, both operands K-major.
 __device__ __forceinline__ uint32_t instruction_f8(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 
-__device__ __forceinline__ void tmem_load_16(uint32_t address, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(address)
-        : "memory");
+// One lane of the warp, chosen by the hardware.  What it issues is then known to come from one thread, with operands that the whole
+// warp shares: under `lane == 0` each MMA and copy cost 70 to 200 cycles more, and a unit 880 however small.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    return elected != 0;
 }
 
-// 4 bytes from global to shared memory (zeros where `present` is false), and this thread's arrival on a barrier once all its copies
-// so far have landed.
-__device__ __forceinline__ void copy_4(uint32_t dst, const float* src, bool present) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(present ? 4u : 0u) : "memory");
+// COUNT columns of this warp's rows; the caller waits once for all loads that it has issued.
+template <int COUNT>
+__device__ __forceinline__ void tmem_ask(uint32_t address, uint32_t (&r)[COUNT]);
+template <>
+__device__ __forceinline__ void tmem_ask<16>(uint32_t address, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(address) : "memory");
 }
-__device__ __forceinline__ void arrive_when_copied(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+template <>
+__device__ __forceinline__ void tmem_ask<32>(uint32_t address, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+                   "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+                   "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(address) : "memory");
+}
+// The array is an operand, so that nothing reads it before the wait.
+template <int COUNT>
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[COUNT]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) asm volatile("" : "+r"(r[i]));
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -93,27 +122,32 @@ __device__ __forceinline__ void store_result(const BlockParams& p, int token, in
     else reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
 }
 
-constexpr int buffers_of(int tokens) { return 256 / tokens < kMaxBuffers ? 256 / tokens : kMaxBuffers; }
 constexpr uint32_t stage_bytes(int tokens) { return kWBytes + (uint32_t)tokens * kBlock; }
+// Warps that scale and add, and how many of its tokens one takes at a time: a thread holds its sums and those results side by side.
+constexpr int adders_of(int tokens) { return tokens <= 64 ? 4 : 8; }
+constexpr int threads_of(int tokens) { return 128 + 32 * adders_of(tokens); }
+// Up to 64 tokens two blocks share an SM: one streams while the other begins or ends.  With 128 the registers are only enough for one.
+constexpr int per_sm_of(int tokens) { return tokens <= 64 ? 2 : 1; }
+constexpr int buffers_of(int tokens) { return 512 / per_sm_of(tokens) / tokens < kMaxBuffers ? 512 / per_sm_of(tokens) / tokens : kMaxBuffers; }
 
-// Up to 64 tokens two blocks share an SM; with 128 a thread's sums alone are 128 registers, and a block has the SM to itself.
 template <int TOKENS>
-__global__ void __launch_bounds__(kThreads, TOKENS <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
     gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const BlockParams p) {
     constexpr int kBuffers = buffers_of(TOKENS);
     constexpr uint32_t kColumns = kBuffers * TOKENS;
     constexpr uint32_t kStageBytes = stage_bytes(TOKENS);
+    constexpr int kAdders = adders_of(TOKENS), kWidth = TOKENS * 4 / kAdders, kPart = kWidth < 32 ? kWidth : 32;      // a warp's tokens, at a time
     extern __shared__ unsigned char block_shared[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], sums_full[kMaxBuffers], sums_empty[kMaxBuffers],
         scale_full[kScaleSlots], scale_empty[kScaleSlots];
-    __shared__ __align__(16) float token_scales[kScaleSlots][TOKENS];
+    __shared__ __align__(16) float scales[kScaleSlots][TOKENS];      // of a unit: each token's times W's
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
     const uint32_t ring = (tma::smem_u32(block_shared) + 1023u) & ~1023u;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = p.split > 1 ? (int)cluster_rank() : 0;
     const int tile = blockIdx.x / p.split, token0 = blockIdx.y * TOKENS;
-    const int first = (int)((long long)p.groups * rank / p.split), count = (int)((long long)p.groups * (rank + 1) / p.split) - first;
+    const int first = p.groups * rank / p.split, count = p.groups * (rank + 1) / p.split - first;      // this block's units
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
@@ -122,11 +156,11 @@ __global__ void __launch_bounds__(kThreads, TOKENS <= 64 ? 2 : 1)
         }
         for (int b = 0; b < kBuffers; ++b) {
             tma::mbar_init(tma::smem_u32(&sums_full[b]), 1);
-            tma::mbar_init(tma::smem_u32(&sums_empty[b]), 4);
+            tma::mbar_init(tma::smem_u32(&sums_empty[b]), kAdders);
         }
         for (int s = 0; s < kScaleSlots; ++s) {
-            tma::mbar_init(tma::smem_u32(&scale_full[s]), 32);
-            tma::mbar_init(tma::smem_u32(&scale_empty[s]), 4);
+            tma::mbar_init(tma::smem_u32(&scale_full[s]), 1);
+            tma::mbar_init(tma::smem_u32(&scale_empty[s]), kAdders);
         }
         tma::mbar_fence_init();
         failed = 0;
@@ -135,6 +169,7 @@ __global__ void __launch_bounds__(kThreads, TOKENS <= 64 ? 2 : 1)
                 tma::mbar_expect_tx(tma::smem_u32(&full[s]), kStageBytes);
                 tma::load_2d(ring + s * kStageBytes, &map_w, tma::smem_u32(&full[s]), (first + s) * kBlock, tile * kRows);
             }
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
     }
     pdl_wait();
     // Tensor memory is taken when the kernel in front has given its own back, and the successor is let in when this block has its share:
@@ -148,102 +183,135 @@ __global__ void __launch_bounds__(kThreads, TOKENS <= 64 ? 2 : 1)
     tc5::fence_after();
     pdl_trigger();
     const uint32_t tmem = tmem_slot;
-    float sums[TOKENS];
-#pragma unroll
-    for (int c = 0; c < TOKENS; ++c) sums[c] = 0.0f;
 
     if (warp == 0) {
-        if (lane == 0) {
-            bool ok = true;
-            for (int i = 0; i < count && ok; ++i) {
-                const int s = i % p.stages;
-                const uint32_t stage = ring + s * kStageBytes, bar = tma::smem_u32(&full[s]);
-                if (i >= p.stages) ok = tma::mbar_wait(tma::smem_u32(&empty[s]), ((i / p.stages) - 1) & 1);
-                if (!ok) break;
+        bool ok = true;
+        Turn turn;
+        for (int i = 0; i < count && ok; ++i) {
+            const uint32_t stage = ring + turn.at * kStageBytes, bar = tma::smem_u32(&full[turn.at]);
+            if (i >= p.stages) ok = __all_sync(0xffffffffu, tma::mbar_wait(tma::smem_u32(&empty[turn.at]), turn.parity ^ 1));
+            if (!ok) break;
+            if (elect_one()) {
                 if (!p.early || i >= p.stages) {
                     tma::mbar_expect_tx(bar, kStageBytes);
                     tma::load_2d(stage, &map_w, bar, (first + i) * kBlock, tile * kRows);
                 }
                 tma::load_2d(stage + kWBytes, &map_x, bar, (first + i) * kBlock, token0);
             }
-            // the last MMAs signal this block's barriers: it may not leave before they have
-            for (int back = count < p.stages ? count : p.stages; back > 0 && ok; --back)
-                ok = tma::mbar_wait(tma::smem_u32(&empty[(count - back) % p.stages]), ((count - back) / p.stages) & 1);
-            if (!ok) failed = 1;
+            turn.step(p.stages);
         }
+        // the last MMAs signal this block's barriers: it may not leave before they have
+        for (int back = count < p.stages ? count : p.stages; back > 0 && ok; --back)
+            ok = tma::mbar_wait(tma::smem_u32(&empty[(count - back) % p.stages]), ((count - back) / p.stages) & 1);
+        if (!ok) failed = 1;
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = instruction_f8(kRows, TOKENS);
-            bool ok = true;
-            for (int i = 0; i < count && ok; ++i) {
-                const int s = i % p.stages, b = i % kBuffers;
-                if (i >= kBuffers) ok = tma::mbar_wait(tma::smem_u32(&sums_empty[b]), ((i / kBuffers) - 1) & 1);
-                if (ok) ok = tma::mbar_wait(tma::smem_u32(&full[s]), (i / p.stages) & 1);
-                if (!ok) break;
-                tc5::fence_after();
-                const uint32_t stage = ring + s * kStageBytes;
-#pragma unroll
-                for (int k = 0; k < kBlock / 32; ++k)
-                    mma_f8(tmem + b * TOKENS, tc5::desc_k_major(stage + k * 32, 1024u), tc5::desc_k_major(stage + kWBytes + k * 32, 1024u), idesc, k > 0);
-                tc5::mma_commit(tma::smem_u32(&empty[s]));
-                tc5::mma_commit(tma::smem_u32(&sums_full[b]));
-            }
-            if (!ok) failed = 1;
-        }
-    } else if (warp == 2) {
+        const uint32_t idesc = instruction_f8(kRows, TOKENS);
+        const uint64_t desc_w = tc5::desc_k_major(ring, 1024u), desc_x = tc5::desc_k_major(ring + kWBytes, 1024u);
         bool ok = true;
+        Turn turn, buffer;
         for (int i = 0; i < count && ok; ++i) {
-            const int s = i % kScaleSlots;
-            if (i >= kScaleSlots) ok = tma::mbar_wait(tma::smem_u32(&scale_empty[s]), ((i / kScaleSlots) - 1) & 1);
+            if (i >= kBuffers) ok = tma::mbar_wait(tma::smem_u32(&sums_empty[buffer.at]), buffer.parity ^ 1);
+            ok = __all_sync(0xffffffffu, ok && tma::mbar_wait(tma::smem_u32(&full[turn.at]), turn.parity));
             if (!ok) break;
-            for (int t = lane; t < TOKENS; t += 32) {
-                const bool present = token0 + t < p.m;
-                copy_4(tma::smem_u32(&token_scales[s][t]), p.x_scales + (present ? (size_t)(token0 + t) * p.groups + first + i : 0), present);
+            tc5::fence_after();
+            const uint64_t stage = turn.at * (kStageBytes >> 4);      // descriptors hold addresses in units of 16 bytes
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < kBlock / 32; ++k) mma_f8(tmem + buffer.at * TOKENS, desc_w + stage + k * 2, desc_x + stage + k * 2, idesc, k > 0);
+                tc5::mma_commit(tma::smem_u32(&empty[turn.at]));
+                tc5::mma_commit(tma::smem_u32(&sums_full[buffer.at]));
             }
-            arrive_when_copied(tma::smem_u32(&scale_full[s]));
+            turn.step(p.stages);
+            buffer.step(kBuffers);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (!ok) failed = 1;
+        } else if (warp == 2) {
+        // A lane's tokens' scales times W's, asked for kScalesAhead units before.
+        constexpr int kMine = TOKENS < 32 ? 1 : TOKENS / 32;
+        const float* w_scales = p.w_scales + (size_t)tile * p.groups + first;
+        float x_scale[kScalesAhead][kMine], w_scale[kScalesAhead];
+        auto ask = [&](int i, float (&x)[kMine], float& w) {
+            w = w_scales[i];
+#pragma unroll
+            for (int t = 0; t < kMine; ++t) {
+                const int token = token0 + t * 32 + lane;
+                x[t] = token < p.m && t * 32 + lane < TOKENS ? p.x_scales[(size_t)token * p.groups + first + i] : 0.0f;
+            }
+        };
+#pragma unroll
+        for (int d = 0; d < kScalesAhead; ++d)
+            if (d < count) ask(d, x_scale[d], w_scale[d]);
+        bool ok = true;
+        Turn slot;
+        for (int i = 0; i < count && ok; i += kScalesAhead) {
+#pragma unroll
+            for (int d = 0; d < kScalesAhead; ++d) {
+                if (i + d >= count || !ok) break;
+                if (i + d >= kScaleSlots) ok = __all_sync(0xffffffffu, tma::mbar_wait(tma::smem_u32(&scale_empty[slot.at]), slot.parity ^ 1));
+                if (!ok) break;
+#pragma unroll
+                for (int t = 0; t < kMine; ++t)
+                    if (t * 32 + lane < TOKENS) scales[slot.at][t * 32 + lane] = x_scale[d][t] * w_scale[d];
+                __syncwarp();
+                if (lane == 0) tma::mbar_arrive(tma::smem_u32(&scale_full[slot.at]));
+                slot.step(kScaleSlots);
+                if (i + d + kScalesAhead < count) ask(i + d + kScalesAhead, x_scale[d], w_scale[d]);
+            }
+        }
         if (!ok) failed = 1;
     } else if (warp >= 4) {
-        const uint32_t address = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const float* w_scales = p.w_scales + (size_t)tile * p.groups + first;
+        const int row = (warp & 3) * 32 + lane, mine = warp < 8 ? 0 : kWidth;      // its row of W in the tile, its first token
+        const uint32_t address = tmem + ((uint32_t)((warp & 3) * 32) << 16) + mine;
+        uint64_t sums[kWidth / 2];      // of two tokens each
+#pragma unroll
+        for (int c = 0; c < kWidth / 2; ++c) sums[c] = 0;
         bool ok = true;
-        float w_scale = count > 0 ? w_scales[0] : 0.0f;
+        Turn slot, buffer;
         for (int i = 0; i < count && ok; ++i) {
-            const int s = i % kScaleSlots, b = i % kBuffers;
-            const float scale = w_scale;
-            if (i + 1 < count) w_scale = w_scales[i + 1];
-            ok = __all_sync(0xffffffffu, tma::mbar_wait(tma::smem_u32(&scale_full[s]), (i / kScaleSlots) & 1) &&
-                                             tma::mbar_wait(tma::smem_u32(&sums_full[b]), (i / kBuffers) & 1));
+            ok = __all_sync(0xffffffffu, tma::mbar_wait(tma::smem_u32(&scale_full[slot.at]), slot.parity) &&
+                                             tma::mbar_wait(tma::smem_u32(&sums_full[buffer.at]), buffer.parity));
             if (!ok) break;
             tc5::fence_after();
 #pragma unroll
-            for (int part = 0; part < TOKENS / 16; ++part) {
-                uint32_t r[16];
-                tmem_load_16(address + b * TOKENS + part * 16, r);
+            for (int part = 0; part < kWidth; part += kPart) {
+                uint32_t r[kPart];
+                tmem_ask<kPart>(address + buffer.at * TOKENS + part, r);
+                tmem_wait<kPart>(r);
+                if (part + kPart == kWidth) {      // all of the buffer is in registers
+                    tc5::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tma::mbar_arrive(tma::smem_u32(&sums_empty[buffer.at]));
+                }
 #pragma unroll
-                for (int c = 0; c < 16; ++c)
-                    sums[part * 16 + c] = fmaf(__uint_as_float(r[c]), token_scales[s][part * 16 + c] * scale, sums[part * 16 + c]);
+                for (int c = 0; c < kPart; c += 4) {
+                    const ulonglong2 scale = *reinterpret_cast<const ulonglong2*>(&scales[slot.at][mine + part + c]);
+                    uint64_t& low = sums[(part + c) / 2];
+                    uint64_t& high = sums[(part + c) / 2 + 1];
+                    low = tc5::fma_pair(tc5::pair_of(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale.x, low);
+                    high = tc5::fma_pair(tc5::pair_of(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale.y, high);
+                }
             }
-            tc5::fence_before();
             __syncwarp();
-            if (lane == 0) {
-                tma::mbar_arrive(tma::smem_u32(&sums_empty[b]));
-                tma::mbar_arrive(tma::smem_u32(&scale_empty[s]));
-            }
+            if (lane == 0) tma::mbar_arrive(tma::smem_u32(&scale_empty[slot.at]));
+            slot.step(kScaleSlots);
+            buffer.step(kBuffers);
         }
         if (!ok) failed = 1;
-        const int row = (warp & 3) * 32 + lane;
-        if (p.split == 1) {
-            if (tile * kRows + row < p.n)
+        const int w_row = tile * kRows + row;
 #pragma unroll
-                for (int c = 0; c < TOKENS; ++c)
-                    if (token0 + c < p.m) store_result(p, token0 + c, tile * kRows + row, sums[c]);
-        } else if (ok) {
-            // all copies into the ring and all MMAs that read it are complete: [token][row of W]
-#pragma unroll
-            for (int c = 0; c < TOKENS; ++c)
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + (c * kRows + row) * 4), "f"(sums[c]) : "memory");
+        for (int c = 0; c < kWidth; c += 2) {
+            float low, high;
+            tc5::halves_of(sums[c / 2], low, high);
+            if (p.split > 1) {
+                // all copies into the ring and all MMAs that read it are complete: [token][row of W]
+                if (ok) {
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + ((mine + c) * kRows + row) * 4), "f"(low) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + ((mine + c + 1) * kRows + row) * 4), "f"(high) : "memory");
+                }
+            } else if (w_row < p.n) {
+                if (token0 + mine + c < p.m) store_result(p, token0 + mine + c, w_row, low);
+                if (token0 + mine + c + 1 < p.m) store_result(p, token0 + mine + c + 1, w_row, high);
+            }
         }
     }
     __syncwarp();
@@ -255,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, TOKENS <= 64 ? 2 : 1)
     if (p.split > 1) {
         cluster_sync();
         // the tokens of a tile are dealt to the blocks of the cluster, a warp each
-        for (int t = rank + warp * p.split; t < TOKENS && token0 + t < p.m; t += kThreads / 32 * p.split) {
+        for (int t = rank + warp * p.split; t < TOKENS && token0 + t < p.m; t += threads_of(TOKENS) / 32 * p.split) {
             float4 sum = load_peer4(ring + (t * kRows + lane * 4) * 4, 0);
             for (int peer = 1; peer < p.split; ++peer) {
                 const float4 part = load_peer4(ring + (t * kRows + lane * 4) * 4, peer);
@@ -284,6 +352,18 @@ bool make_map_f8(CUtensorMap* map, const void* pointer, uint64_t rows, uint64_t 
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int tokens_per_tile(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
+
+// Into how many parts k is split: as many as one round of blocks holds (a second round waits for the first to give up its share of an SM:
+// 1 row by 24576 x 4096, 192 tiles on 296 places, 19.1 us whole, 23.4 in two parts, 26.6 in three), a power of two (clusters of 3, 5, 6 and 7 leave
+// places empty: 1 row by 6144 x 4096 in four parts 8.3 us, in six 12.5), each of two units at least.
+int split_of(long long tiles, int groups, int per_sm) {
+    const long long room = (long long)per_sm * llm_sm_count();
+    int split = 1;
+    while (2 * split <= kMaxSplit && tiles * 2 * split <= room && groups / (2 * split) >= 2) split *= 2;
+    return split;
+}
+
 template <int TOKENS>
 int launch_block_scaled(const void* x, long long x_pitch, const void* w, long long w_pitch, BlockParams p, int inner, cudaStream_t stream) {
     CUtensorMap map_w, map_x;
@@ -293,18 +373,14 @@ int launch_block_scaled(const void* x, long long x_pitch, const void* w, long lo
         return LLM_REFUSED;
     }
     const int tiles = (p.n + kRows - 1) / kRows, token_tiles = (p.m + TOKENS - 1) / TOKENS;
-    const int per_sm = TOKENS <= 64 ? 2 : 1;
-    const long long room = (long long)per_sm * llm_sm_count();
-    p.split = 1;
-    while (2 * p.split <= kMaxSplit && (long long)tiles * token_tiles * 2 * p.split <= room && p.groups / (2 * p.split) >= 2) p.split *= 2;
-    const uint32_t ring_bytes = per_sm == 2 ? 96u << 10 : 200u << 10;
+    p.split = split_of((long long)tiles * token_tiles, p.groups, per_sm_of(TOKENS));
+    const uint32_t ring_bytes = per_sm_of(TOKENS) == 2 ? 96u << 10 : 200u << 10;
     p.stages = (int)(ring_bytes / stage_bytes(TOKENS));
-    if (p.stages > kMaxStages) p.stages = kMaxStages;
-    size_t shared = (size_t)p.stages * stage_bytes(TOKENS) + 1024;
+    const size_t shared = (size_t)p.stages * stage_bytes(TOKENS) + 1024;
     if (int status = llm_raise_shared_limit((const void*)gemm_block_scaled_kernel<TOKENS>, shared, "block_linear", true)) return status;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(tiles * p.split), (unsigned)token_tiles, 1);
-    config.blockDim = dim3(kThreads, 1, 1);
+    config.blockDim = dim3(threads_of(TOKENS), 1, 1);
     config.dynamicSmemBytes = shared;
     config.stream = stream;
     cudaLaunchAttribute attribute[2];
@@ -324,38 +400,61 @@ int launch_block_scaled(const void* x, long long x_pitch, const void* w, long lo
     return llm_check_launch("block_linear");
 }
 
+int refuse_product(long long m, int n, int inner, long long x_pitch, long long w_pitch) {
+    if (m < 0 || n < 1 || inner < 1 || x_pitch < inner || x_pitch % 16 != 0 || w_pitch < inner || w_pitch % 16 != 0 || m > 65535 * 128LL ||
+        (n + 127LL) / 128 * kMaxSplit > 0x7fffffffLL) {
+        llm_set_error("block_linear: [%lld, %d] x [%d, %d]^T with rows %lld and %lld bytes apart is not supported", m, inner, n, inner, x_pitch, w_pitch);
+        return LLM_REFUSED;
+    }
+    return LLM_OK;
+}
+
 }  // namespace
 
 extern "C" int llm_quantize_blocks(const void* x, int dtype, void* out, float* scales, int rows, int inner, long long pitch, int block_rows,
                                    cudaStream_t stream);
 
-// out[m, n] (float or bfloat16) = x W^T.  `x` [m, inner] float or bfloat16 (x_dtype), brought to 8 bits in xq [m, x_pitch] and
-// x_scales [m, ceil(inner / 128)] first; null: xq and x_scales hold it already.
-LLM_EXPORT int llm_block_linear(const void* x, int x_dtype, void* xq, long long x_pitch, float* x_scales, const void* w, long long w_pitch,
-                                const float* w_scales, void* out, int out_is_f32, int m, int n, int inner, int* error_flag, cudaStream_t stream) {
-    if (m < 0 || n < 1 || inner < 1 || x_pitch < inner || x_pitch % 16 != 0 || w_pitch < inner || w_pitch % 16 != 0 || !aligned16(xq) || !aligned16(w)) {
-        llm_set_error("block_linear: [%d, %d] x [%d, %d]^T with rows %lld and %lld bytes apart is not supported", m, inner, n, inner, x_pitch, w_pitch);
+// out[m, n] (float or bfloat16) = x W^T.  `x` [m, inner]: float or bfloat16 (x_dtype 0 or 1, contiguous), or (x_dtype -1) 8 bits with rows
+// x_pitch bytes apart and x_scales [m, ceil(inner / 128)].  The former are brought to 8 bits in `scratch`: m rows of x_pitch bytes, then
+// m * ceil(inner / 128) scales.
+LLM_EXPORT int llm_block_linear(const void* x, int x_dtype, long long x_pitch, const float* x_scales, const void* w, long long w_pitch,
+                                const float* w_scales, void* out, int out_is_f32, int m, int n, int inner, void* scratch, int* error_flag,
+                                cudaStream_t stream) {
+    if (int status = refuse_product(m, n, inner, x_pitch, w_pitch)) return status;
+    if (!aligned16(w) || (x_dtype < 0 && !aligned16(x)) || !aligned16(scratch)) {
+        llm_set_error("block_linear: operands in 8 bits begin at multiples of 16 bytes");
+        return LLM_REFUSED;
+    }
+    if (x_dtype >= 0 && m > 0 && scratch == nullptr) {
+        llm_set_error("block_linear: %d rows are brought to 8 bits in scratch, and there is none", m);
+        return LLM_REFUSED;
+    }
+    if (x_dtype > LLM_BF16) {
+        llm_set_error("unknown dtype code %d", x_dtype);
         return LLM_REFUSED;
     }
     if (m == 0) return LLM_OK;
-    if (m > 65535 * 128) {
-        llm_set_error("block_linear: at most %d rows, got %d", 65535 * 128, m);
-        return LLM_REFUSED;
-    }
-    if (x != nullptr)
-        if (int status = llm_quantize_blocks(x, x_dtype, xq, x_scales, m, inner, x_pitch, 1, stream)) return status;
     BlockParams p = {};
+    p.groups = (inner + kBlock - 1) / kBlock;
     p.x_scales = x_scales;
     p.w_scales = w_scales;
     p.out = out;
     p.out_is_f32 = out_is_f32;
     p.m = m;
     p.n = n;
-    p.groups = (inner + kBlock - 1) / kBlock;
-    p.early = x != nullptr;
     p.error_flag = error_flag;
-    if (m <= 16) return launch_block_scaled<16>(xq, x_pitch, w, w_pitch, p, inner, stream);
-    if (m <= 32) return launch_block_scaled<32>(xq, x_pitch, w, w_pitch, p, inner, stream);
-    if (m <= 64) return launch_block_scaled<64>(xq, x_pitch, w, w_pitch, p, inner, stream);
-    return launch_block_scaled<128>(xq, x_pitch, w, w_pitch, p, inner, stream);
+    const void* rows = x;
+    if (x_dtype >= 0) {
+        float* made = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + (size_t)m * x_pitch);
+        if (int status = llm_quantize_blocks(x, x_dtype, scratch, made, m, inner, x_pitch, 1, stream)) return status;
+        rows = scratch;
+        p.x_scales = made;
+        p.early = 1;      // that kernel lets this one in only when all in front of it is complete
+    }
+    switch (tokens_per_tile(m)) {
+        case 16: return launch_block_scaled<16>(rows, x_pitch, w, w_pitch, p, inner, stream);
+        case 32: return launch_block_scaled<32>(rows, x_pitch, w, w_pitch, p, inner, stream);
+        case 64: return launch_block_scaled<64>(rows, x_pitch, w, w_pitch, p, inner, stream);
+        default: return launch_block_scaled<128>(rows, x_pitch, w, w_pitch, p, inner, stream);
+    }
 }

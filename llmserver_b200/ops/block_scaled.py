@@ -145,14 +145,13 @@ def block_linear(x, weight: BlockScaled, out: Optional[torch.Tensor] = None, out
         out = torch.empty((rows, cols), dtype=out_dtype, device=device)
     elif out.dtype != out_dtype or not out.is_contiguous() or tuple(out.shape) != (rows, cols):
         raise KernelError(f"block_linear: the output must be contiguous {out_dtype} [{rows}, {cols}], got {out.dtype} {tuple(out.shape)}")
+    scratch = 0
     if quantized:
-        source, kind, values, pitch, scales = 0, 0, x.values.data_ptr(), _row_stride(x.values), x.scales.data_ptr()
+        kind, pitch, scales, source = -1, _row_stride(x.values), x.scales.data_ptr(), x.values.data_ptr()
     else:
-        # one piece of scratch: the rows' 8-bit numbers, then their scales
-        pitch = _pitch(inner)
-        scratch = torch.empty(rows * (pitch + 4 * _blocks(inner)), dtype=torch.uint8, device=device)
-        source, kind, values = x.data_ptr(), dtype_code(x.dtype), scratch.data_ptr()
-        scales = values + rows * pitch
-    call("llm_block_linear", source, kind, values, pitch, scales, weight.values.data_ptr(), _row_stride(weight.values), weight.scales.data_ptr(),
-         out.data_ptr(), int(out_dtype == torch.float32), rows, cols, inner, wait_error_flag(device).data_ptr(), stream_handle())
+        kind, pitch, scales, source = dtype_code(x.dtype), _pitch(inner), 0, x.data_ptr()
+        room = torch.empty(rows * (pitch + 4 * _blocks(inner)), dtype=torch.uint8, device=device)      # the rows in 8 bits, then their scales
+        scratch = room.data_ptr()
+    call("llm_block_linear", source, kind, pitch, scales, weight.values.data_ptr(), _row_stride(weight.values), weight.scales.data_ptr(),
+         out.data_ptr(), int(out_dtype == torch.float32), rows, cols, inner, scratch, wait_error_flag(device).data_ptr(), stream_handle())
     return out

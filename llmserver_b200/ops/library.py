@@ -32,7 +32,7 @@ SIGNATURES = {
     "llm_control_logits": [_P, _P, _I, _I, _P, _S],
     "llm_control_sample": [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _S],
     "llm_quantize_blocks": [_P, _I, _P, _P, _I, _I, ctypes.c_longlong, _I, _S],
-    "llm_block_linear": [_P, _I, _P, ctypes.c_longlong, _P, _P, ctypes.c_longlong, _P, _P, _I, _I, _I, _I, _P, _S],
+    "llm_block_linear": [_P, _I, ctypes.c_longlong, _P, _P, ctypes.c_longlong, _P, _P, _I, _I, _I, _I, _P, _P, _S],
     "llm_qk_norm_rope_kv_write": [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _I, _I, _I, _S],
     "llm_attention_generic": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _I, _S],
     "llm_rope_kv_write_split": [_P, _P, _F, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I, _I, _S],

@@ -36,14 +36,14 @@ def test_the_launcher_refuses_sizes_it_cannot_take(rows, inner, pitch, block_row
 def test_the_product_refuses_sizes_it_cannot_take():
     library = ops.library()
 
-    def run(m=1, n=128, inner=128, x_pitch=128, w_pitch=128, xq=0, w=0):
-        return library.llm_block_linear(0, 0, xq, x_pitch, 0, w, w_pitch, 0, 0, 0, m, n, inner, 0, 0)
+    def run(m=1, n=128, inner=128, x_pitch=128, w_pitch=128, x=0, w=0, scratch=0, dtype=-1):
+        return library.llm_block_linear(x, dtype, x_pitch, 0, w, w_pitch, 0, 0, 0, m, n, inner, scratch, 0, 0)
 
     assert run(m=0) == 0
-    for given in ({"m": -1}, {"n": 0}, {"inner": 0}, {"x_pitch": 120}, {"w_pitch": 120}, {"x_pitch": 112}, {"w_pitch": 112}, {"xq": 8}, {"w": 4},
-                  {"m": 65535 * 128 + 1}):
+    for given in ({"m": -1}, {"n": 0}, {"inner": 0}, {"x_pitch": 120}, {"w_pitch": 120}, {"x_pitch": 112}, {"w_pitch": 112}, {"x": 8}, {"w": 4},
+                  {"m": 65535 * 128 + 1}, {"scratch": 8}, {"dtype": 2}, {"dtype": 0}):
         assert run(**given) == -1, given
-        assert b"block_linear" in library.llm_last_error()
+        assert library.llm_last_error()
 
 
 def test_dtype_codes_are_checked_before_a_launch():
