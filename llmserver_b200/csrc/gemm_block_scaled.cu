@@ -5,8 +5,8 @@
 // multiplied with the block's two scales and added up in registers, 32-bit as well: the scales are any 32-bit numbers, so blocks
 // cannot be added before they are scaled.
 //
-// The roles of the operands are swapped for the hardware, as in gemm_tcgen05.cu: 128 rows of W are the MMA's M, the tokens (16 to
-// 128) its N, so that a product of few tokens streams W and wastes nothing on rows that do not exist.  A stage of the ring is one
+// For up to 64 tokens (more: gemm_block_scaled_many.cu).  The roles of the operands are swapped for the hardware, as in gemm_tcgen05.cu:
+// 128 rows of W are the MMA's M, the tokens (16, 32 or 64) its N, so that a product of few tokens streams W and wastes nothing on rows that do not exist.  A stage of the ring is one
 // block of 128 along k: 16 KiB of W and up to 16 KiB of x, which are one swizzle atom wide.  The MMAs of a block go to one of several
 // buffers of tensor memory, so that they run ahead of the warps that scale and add.
 //
@@ -14,20 +14,24 @@
 // the order of k (see split_of).
 //
 // Roles: warp 0 copies (TMA), warp 1 issues the MMAs, warp 2 leaves each unit's scales (a token's times W's) in shared
-// memory, warp 3 holds the tensor memory, and the other four or eight scale and add, a row of W and up to 64 tokens per thread.  All waits are
+// memory, warp 3 holds the tensor memory, and the other four scale and add, a row of W per thread.  All waits are
 // bounded: one that runs out sets error code 2, every role leaves its loop, and the block still frees its tensor memory and meets its
 // cluster.
 //
 // k need not be a multiple of 128 nor n of 128 nor m of anything: what lies outside is read as zeros (TMA) and not written.
-#include "block_scaled.cuh"
-#include "tcgen05.cuh"
-#include "tma.cuh"
+#include "block_scaled_mma.cuh"
 
 namespace {
 
+using namespace block_scaled;
+
 constexpr int kRows = 128;            // rows of W per tile (UMMA M)
-using block_scaled::kBlock;           // of k: one stage of the ring, one pair of scales
-constexpr int kMaxStages = 12;
+constexpr int kMany = 64;             // beyond so many tokens they are the MMA's M (gemm_block_scaled_many.cu)
+constexpr int kAdders = 4;            // warps that scale and add
+constexpr int kThreads = 128 + 32 * kAdders;
+constexpr int kPerSm = 2;             // blocks that share an SM: one streams while the other begins or ends
+constexpr uint32_t kRingBytes = 96 << 10;
+constexpr int kMaxStages = 6;
 constexpr int kMaxSplit = 8;
 constexpr int kScaleSlots = 8;        // units whose scales wait to be used
 constexpr int kScalesAhead = 4;       // and those on their way from memory
@@ -45,77 +49,6 @@ struct BlockParams {
     int* error_flag;
 };
 
-// A place in a ring and the parity of its turn.  It moves by additions: a division of integers is a hundred cycles for a role that one warp
-// plays, and with five of them per unit a unit took 1150 cycles, whatever its size.
-struct Turn {
-    int at = 0;
-    uint32_t parity = 0;
-    __device__ __forceinline__ void step(int size) {
-        if (++at == size) at = 0, parity ^= 1;
-    }
-};
-
-__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// e4m3 x e4m3 -> float32, both operands K-major.
-__device__ __forceinline__ uint32_t instruction_f8(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
-
-// One lane of the warp, chosen by the hardware.  What it issues is then known to come from one thread, with operands that the whole
-// warp shares: under `lane == 0` each MMA and copy cost 70 to 200 cycles more, and a unit 880 however small.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t elected;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
-    return elected != 0;
-}
-
-// COUNT columns of this warp's rows; the caller waits once for all loads that it has issued.
-template <int COUNT>
-__device__ __forceinline__ void tmem_ask(uint32_t address, uint32_t (&r)[COUNT]);
-template <>
-__device__ __forceinline__ void tmem_ask<16>(uint32_t address, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(address) : "memory");
-}
-template <>
-__device__ __forceinline__ void tmem_ask<32>(uint32_t address, uint32_t (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-                   "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-                   "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(address) : "memory");
-}
-// The array is an operand, so that nothing reads it before the wait.
-template <int COUNT>
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[COUNT]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) asm volatile("" : "+r"(r[i]));
-}
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t rank;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    return rank;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float4 load_peer4(uint32_t local_address, uint32_t rank) {
-    uint32_t remote;
-    float4 value;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_address), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(value.x), "=f"(value.y), "=f"(value.z), "=f"(value.w) : "r"(remote) : "memory");
-    return value;
-}
-
 __device__ __forceinline__ void store_result(const BlockParams& p, int token, int row, float v) {
     const size_t at = (size_t)token * p.n + row;
     if (p.out_is_f32) reinterpret_cast<float*>(p.out)[at] = v;
@@ -123,20 +56,15 @@ __device__ __forceinline__ void store_result(const BlockParams& p, int token, in
 }
 
 constexpr uint32_t stage_bytes(int tokens) { return kWBytes + (uint32_t)tokens * kBlock; }
-// Warps that scale and add, and how many of its tokens one takes at a time: a thread holds its sums and those results side by side.
-constexpr int adders_of(int tokens) { return tokens <= 64 ? 4 : 8; }
-constexpr int threads_of(int tokens) { return 128 + 32 * adders_of(tokens); }
-// Up to 64 tokens two blocks share an SM: one streams while the other begins or ends.  With 128 the registers are only enough for one.
-constexpr int per_sm_of(int tokens) { return tokens <= 64 ? 2 : 1; }
-constexpr int buffers_of(int tokens) { return 512 / per_sm_of(tokens) / tokens < kMaxBuffers ? 512 / per_sm_of(tokens) / tokens : kMaxBuffers; }
+constexpr int buffers_of(int tokens) { return 256 / tokens < kMaxBuffers ? 256 / tokens : kMaxBuffers; }
 
 template <int TOKENS>
-__global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
+__global__ void __launch_bounds__(kThreads, kPerSm)
     gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const BlockParams p) {
     constexpr int kBuffers = buffers_of(TOKENS);
     constexpr uint32_t kColumns = kBuffers * TOKENS;
     constexpr uint32_t kStageBytes = stage_bytes(TOKENS);
-    constexpr int kAdders = adders_of(TOKENS), kWidth = TOKENS * 4 / kAdders, kPart = kWidth < 32 ? kWidth : 32;      // a warp's tokens, at a time
+    constexpr int kPart = TOKENS < 32 ? TOKENS : 32;      // tokens read from tensor memory at a time
     extern __shared__ unsigned char block_shared[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], sums_full[kMaxBuffers], sums_empty[kMaxBuffers],
         scale_full[kScaleSlots], scale_empty[kScaleSlots];
@@ -146,7 +74,7 @@ __global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
     const uint32_t ring = (tma::smem_u32(block_shared) + 1023u) & ~1023u;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = p.split > 1 ? (int)cluster_rank() : 0;
-    const int tile = blockIdx.x / p.split, token0 = blockIdx.y * TOKENS;
+    const int tile = blockIdx.x / p.split;
     const int first = p.groups * rank / p.split, count = p.groups * (rank + 1) / p.split - first;      // this block's units
 
     if (threadIdx.x == 0) {
@@ -196,7 +124,7 @@ __global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
                     tma::mbar_expect_tx(bar, kStageBytes);
                     tma::load_2d(stage, &map_w, bar, (first + i) * kBlock, tile * kRows);
                 }
-                tma::load_2d(stage + kWBytes, &map_x, bar, (first + i) * kBlock, token0);
+                tma::load_2d(stage + kWBytes, &map_x, bar, (first + i) * kBlock, 0);
             }
             turn.step(p.stages);
         }
@@ -234,7 +162,7 @@ __global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
             w = w_scales[i];
 #pragma unroll
             for (int t = 0; t < kMine; ++t) {
-                const int token = token0 + t * 32 + lane;
+                const int token = t * 32 + lane;
                 x[t] = token < p.m && t * 32 + lane < TOKENS ? p.x_scales[(size_t)token * p.groups + first + i] : 0.0f;
             }
         };
@@ -260,11 +188,11 @@ __global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
         }
         if (!ok) failed = 1;
     } else if (warp >= 4) {
-        const int row = (warp & 3) * 32 + lane, mine = warp < 8 ? 0 : kWidth;      // its row of W in the tile, its first token
-        const uint32_t address = tmem + ((uint32_t)((warp & 3) * 32) << 16) + mine;
-        uint64_t sums[kWidth / 2];      // of two tokens each
+        const int row = (warp & 3) * 32 + lane;      // its row of W in the tile
+        const uint32_t address = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        uint64_t sums[TOKENS / 2];      // of two tokens each
 #pragma unroll
-        for (int c = 0; c < kWidth / 2; ++c) sums[c] = 0;
+        for (int c = 0; c < TOKENS / 2; ++c) sums[c] = 0;
         bool ok = true;
         Turn slot, buffer;
         for (int i = 0; i < count && ok; ++i) {
@@ -273,18 +201,18 @@ __global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
             if (!ok) break;
             tc5::fence_after();
 #pragma unroll
-            for (int part = 0; part < kWidth; part += kPart) {
+            for (int part = 0; part < TOKENS; part += kPart) {
                 uint32_t r[kPart];
                 tmem_ask<kPart>(address + buffer.at * TOKENS + part, r);
                 tmem_wait<kPart>(r);
-                if (part + kPart == kWidth) {      // all of the buffer is in registers
+                if (part + kPart == TOKENS) {      // all of the buffer is in registers
                     tc5::fence_before();
                     __syncwarp();
                     if (lane == 0) tma::mbar_arrive(tma::smem_u32(&sums_empty[buffer.at]));
                 }
 #pragma unroll
                 for (int c = 0; c < kPart; c += 4) {
-                    const ulonglong2 scale = *reinterpret_cast<const ulonglong2*>(&scales[slot.at][mine + part + c]);
+                    const ulonglong2 scale = *reinterpret_cast<const ulonglong2*>(&scales[slot.at][part + c]);
                     uint64_t& low = sums[(part + c) / 2];
                     uint64_t& high = sums[(part + c) / 2 + 1];
                     low = tc5::fma_pair(tc5::pair_of(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale.x, low);
@@ -299,18 +227,18 @@ __global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
         if (!ok) failed = 1;
         const int w_row = tile * kRows + row;
 #pragma unroll
-        for (int c = 0; c < kWidth; c += 2) {
+        for (int c = 0; c < TOKENS; c += 2) {
             float low, high;
             tc5::halves_of(sums[c / 2], low, high);
             if (p.split > 1) {
                 // all copies into the ring and all MMAs that read it are complete: [token][row of W]
                 if (ok) {
-                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + ((mine + c) * kRows + row) * 4), "f"(low) : "memory");
-                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + ((mine + c + 1) * kRows + row) * 4), "f"(high) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + (c * kRows + row) * 4), "f"(low) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + ((c + 1) * kRows + row) * 4), "f"(high) : "memory");
                 }
             } else if (w_row < p.n) {
-                if (token0 + mine + c < p.m) store_result(p, token0 + mine + c, w_row, low);
-                if (token0 + mine + c + 1 < p.m) store_result(p, token0 + mine + c + 1, w_row, high);
+                if (c < p.m) store_result(p, c, w_row, low);
+                if (c + 1 < p.m) store_result(p, c + 1, w_row, high);
             }
         }
     }
@@ -323,7 +251,7 @@ __global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
     if (p.split > 1) {
         cluster_sync();
         // the tokens of a tile are dealt to the blocks of the cluster, a warp each
-        for (int t = rank + warp * p.split; t < TOKENS && token0 + t < p.m; t += threads_of(TOKENS) / 32 * p.split) {
+        for (int t = rank + warp * p.split; t < TOKENS && t < p.m; t += kThreads / 32 * p.split) {
             float4 sum = load_peer4(ring + (t * kRows + lane * 4) * 4, 0);
             for (int peer = 1; peer < p.split; ++peer) {
                 const float4 part = load_peer4(ring + (t * kRows + lane * 4) * 4, peer);
@@ -332,7 +260,7 @@ __global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
             const float values[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                if (tile * kRows + lane * 4 + c < p.n) store_result(p, token0 + t, tile * kRows + lane * 4 + c, values[c]);
+                if (tile * kRows + lane * 4 + c < p.n) store_result(p, t, tile * kRows + lane * 4 + c, values[c]);
         }
         cluster_sync();      // nobody leaves while others read its shared memory
     }
@@ -340,25 +268,13 @@ __global__ void __launch_bounds__(threads_of(TOKENS), per_sm_of(TOKENS))
     if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns));
 }
 
-// Tensor map of bytes [rows, columns] with `pitch` bytes between rows, box = [box_rows, 128 columns], 128-byte swizzle, zeros outside.
-bool make_map_f8(CUtensorMap* map, const void* pointer, uint64_t rows, uint64_t columns, uint64_t pitch, uint32_t box_rows) {
-    tma::EncodeTiled encode = tma::encode_tiled();
-    if (encode == nullptr) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)pitch};
-    const cuuint32_t box[2] = {(cuuint32_t)kBlock, box_rows};
-    const cuuint32_t ones[2] = {1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pointer), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-int tokens_per_tile(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
+int tokens_per_tile(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
 
 // Into how many parts k is split: as many as one round of blocks holds (a second round waits for the first to give up its share of an SM:
 // 1 row by 24576 x 4096, 192 tiles on 296 places, 19.1 us whole, 23.4 in two parts, 26.6 in three), a power of two (clusters of 3, 5, 6 and 7 leave
 // places empty: 1 row by 6144 x 4096 in four parts 8.3 us, in six 12.5), each of two units at least.
-int split_of(long long tiles, int groups, int per_sm) {
-    const long long room = (long long)per_sm * llm_sm_count();
+int split_of(long long tiles, int groups) {
+    const long long room = (long long)kPerSm * llm_sm_count();
     int split = 1;
     while (2 * split <= kMaxSplit && tiles * 2 * split <= room && groups / (2 * split) >= 2) split *= 2;
     return split;
@@ -372,15 +288,14 @@ int launch_block_scaled(const void* x, long long x_pitch, const void* w, long lo
         llm_set_error("block_linear: the tensor maps could not be made");
         return LLM_REFUSED;
     }
-    const int tiles = (p.n + kRows - 1) / kRows, token_tiles = (p.m + TOKENS - 1) / TOKENS;
-    p.split = split_of((long long)tiles * token_tiles, p.groups, per_sm_of(TOKENS));
-    const uint32_t ring_bytes = per_sm_of(TOKENS) == 2 ? 96u << 10 : 200u << 10;
-    p.stages = (int)(ring_bytes / stage_bytes(TOKENS));
+    const int tiles = (p.n + kRows - 1) / kRows;
+    p.split = split_of(tiles, p.groups);
+    p.stages = (int)(kRingBytes / stage_bytes(TOKENS));
     const size_t shared = (size_t)p.stages * stage_bytes(TOKENS) + 1024;
     if (int status = llm_raise_shared_limit((const void*)gemm_block_scaled_kernel<TOKENS>, shared, "block_linear", true)) return status;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(tiles * p.split), (unsigned)token_tiles, 1);
-    config.blockDim = dim3(threads_of(TOKENS), 1, 1);
+    config.gridDim = dim3((unsigned)(tiles * p.split), 1, 1);
+    config.blockDim = dim3(kThreads, 1, 1);
     config.dynamicSmemBytes = shared;
     config.stream = stream;
     cudaLaunchAttribute attribute[2];
@@ -402,7 +317,7 @@ int launch_block_scaled(const void* x, long long x_pitch, const void* w, long lo
 
 int refuse_product(long long m, int n, int inner, long long x_pitch, long long w_pitch) {
     if (m < 0 || n < 1 || inner < 1 || x_pitch < inner || x_pitch % 16 != 0 || w_pitch < inner || w_pitch % 16 != 0 || m > 65535 * 128LL ||
-        (n + 127LL) / 128 * kMaxSplit > 0x7fffffffLL) {
+        (m + 127) / 128 * ((n + 127LL) / 128) * ((inner + 127LL) / 128) > 0x7fffffffLL / kMaxSplit) {
         llm_set_error("block_linear: [%lld, %d] x [%d, %d]^T with rows %lld and %lld bytes apart is not supported", m, inner, n, inner, x_pitch, w_pitch);
         return LLM_REFUSED;
     }
@@ -411,6 +326,8 @@ int refuse_product(long long m, int n, int inner, long long x_pitch, long long w
 
 }  // namespace
 
+int llm_block_linear_many(const void* x, long long x_pitch, const float* x_scales, const void* w, long long w_pitch, const float* w_scales, void* out,
+                          int out_is_f32, int m, int n, int inner, int early, int* error_flag, cudaStream_t stream);
 extern "C" int llm_quantize_blocks(const void* x, int dtype, void* out, float* scales, int rows, int inner, long long pitch, int block_rows,
                                    cudaStream_t stream);
 
@@ -451,10 +368,11 @@ LLM_EXPORT int llm_block_linear(const void* x, int x_dtype, long long x_pitch, c
         p.x_scales = made;
         p.early = 1;      // that kernel lets this one in only when all in front of it is complete
     }
+    if (m > kMany)
+        return llm_block_linear_many(rows, x_pitch, p.x_scales, w, w_pitch, w_scales, out, out_is_f32, m, n, inner, p.early, error_flag, stream);
     switch (tokens_per_tile(m)) {
         case 16: return launch_block_scaled<16>(rows, x_pitch, w, w_pitch, p, inner, stream);
         case 32: return launch_block_scaled<32>(rows, x_pitch, w, w_pitch, p, inner, stream);
-        case 64: return launch_block_scaled<64>(rows, x_pitch, w, w_pitch, p, inner, stream);
-        default: return launch_block_scaled<128>(rows, x_pitch, w, w_pitch, p, inner, stream);
+        default: return launch_block_scaled<64>(rows, x_pitch, w, w_pitch, p, inner, stream);
     }
 }

@@ -152,7 +152,7 @@ def test_rows_that_begin_anywhere():
 # and many blocks of k, more tiles than SMs
 SIZES = [(1, 128, 128), (1, 1, 1), (2, 16, 5), (15, 127, 129), (16, 129, 128), (17, 500, 257), (32, 512, 1000), (33, 1000, 384), (64, 640, 130),
          (65, 2001, 300), (128, 384, 1111), (129, 1024, 128), (300, 700, 700), (1000, 256, 513), (1, 4096, 6144), (8, 12288, 4096), (61, 4096, 19000),
-         (260, 8192, 260), (511, 1536, 2049)]
+         (260, 8192, 260), (511, 1536, 2049), (66, 300, 40000), (1000, 384, 4100), (1290, 650, 5000), (4500, 130, 1300)]
 
 
 @pytest.mark.parametrize("rows,inner,cols", SIZES)
