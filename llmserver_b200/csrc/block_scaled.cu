@@ -6,85 +6,148 @@
 // since e4m3 is itself a floating format nothing is lost against a scale of max / 448 but half a binade or so below its normal range.  A block
 // that holds an infinity or a NaN (e4m3 has no infinity) becomes NaN whole, values and scale.
 //
-// What bounds it: reading x and writing a byte for each number.  Rows: a warp takes groups of 128 one after the other, four numbers a
-// lane.  Matrices: a block of threads keeps the 128 x 128 numbers in registers between the maximum and the rounding.
+// What bounds it: reading x and writing a byte for each number.  Half a warp takes 128 numbers of a row, eight a lane, as they lie in
+// memory; what a thread needs of x is asked for all at once, before anything is looked at (a branch around each load, for rows that begin
+// anywhere, made the loads wait for one another: 24576 x 4096 bfloat16 in blocks of 128 x 128 took 218 us).  Rows that do not begin at
+// multiples of 16 bytes are read number by number, by kernels of their own.
 #include "block_scaled.cuh"
+
+#include <string.h>
 
 namespace {
 
 using namespace block_scaled;
 
-constexpr int kGroup = kBlock;
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-
-// Numbers 4 i .. 4 i + 3 of a row (those that exist; zeros behind them).  `whole`: the row begins where 4 numbers can be read at once.
+// Eight numbers of a row as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load4(const T* row, int first, int inner, bool whole, float (&v)[4]) {
-    if (whole && first + 4 <= inner) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 raw = *reinterpret_cast<const float4*>(row + first);
-            v[0] = raw.x, v[1] = raw.y, v[2] = raw.z, v[3] = raw.w;
-        } else {
-            const uint2 raw = *reinterpret_cast<const uint2*>(row + first);
-            const float2 low = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
-            const float2 high = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-            v[0] = low.x, v[1] = low.y, v[2] = high.x, v[3] = high.y;
-        }
-    } else {
+struct Eight {
+    uint4 words[sizeof(T) / 2];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = first + c < inner ? Num<T>::load(row + first + c) : 0.0f;
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) words[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void ask(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) words[i] = *(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void ask_singly(const T* row, int first, int inner) {      // those that exist, from wherever the row begins
+        T each[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) Num<T>::store(&each[c], first + c < inner ? Num<T>::load(row + first + c) : 0.0f);
+        memcpy(words, each, sizeof(each));
+    }
+    // The bits of the largest magnitude: as whole numbers magnitudes are ordered, NaN above infinity above all others.
+    __device__ __forceinline__ uint32_t largest() const {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t sign = 0x7fff7fffu;
+            const uint32_t both = __vmaxu2(__vmaxu2(words[0].x & sign, words[0].y & sign), __vmaxu2(words[0].z & sign, words[0].w & sign));
+            return max(both & 0xffff0000u, both << 16);
+        } else {
+            uint32_t found = 0;
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+                found = max(max(found, max(words[i].x & 0x7fffffffu, words[i].y & 0x7fffffffu)), max(words[i].z & 0x7fffffffu, words[i].w & 0x7fffffffu));
+            return found;
+        }
+    }
+    __device__ __forceinline__ uint2 rounded(float inverse) const {
+        float v[8];
+        load8<T>(reinterpret_cast<const T*>(words), v);
+        return make_uint2(four_of(v[0], v[1], v[2], v[3], inverse), four_of(v[4], v[5], v[6], v[7], inverse));
+    }
+};
+
+__device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
+#pragma unroll
+    for (int offset = 8; offset > 0; offset >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, offset));
+    return v;
+}
+
+// The successor may read what does not depend on these kernels as soon as it runs, so it is let in only when everything in front of them is
+// complete.  The rows of `out` begin at multiples of 16 bytes; bytes behind a row's end, up to there, may be written.
+//
+// Rows that are whole groups long: the groups lie one after the other, and half a warp takes kAtOnce of them at a time.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) quantize_groups_kernel(const T* __restrict__ x, unsigned char* __restrict__ out, float* __restrict__ scales,
+                                                                   long long total) {
+    pdl_wait();
+    pdl_trigger();
+    constexpr int kAtOnce = sizeof(T) == 2 ? 4 : 2;
+    const int place = threadIdx.x & 15;
+    const long long halves = (long long)gridDim.x * (kThreads / 16);
+    // (a warp's two halves run side by side to the end: the groups that one of them lacks are left out)
+    for (long long g0 = ((long long)blockIdx.x * kThreads + (threadIdx.x & ~31)) >> 4; g0 < total; g0 += halves * kAtOnce) {
+        const long long first = g0 + ((threadIdx.x >> 4) & 1);
+        Eight<T> numbers[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const long long g = first + i * halves;
+            if (g < total) numbers[i].ask(x + g * kBlock + 8 * place);
+            else numbers[i].clear();
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const long long g = first + i * halves;
+            const Rounding r = rounding_of(half_warp_max(numbers[i].largest()));
+            if (g < total) {
+                *reinterpret_cast<uint2*>(out + g * kBlock + 8 * place) = numbers[i].rounded(r.inverse);
+                if (place == 0) scales[g] = r.scale;
+            }
+        }
     }
 }
 
-// The rows of `out` begin at multiples of 16 bytes; bytes behind a row's end (up to there) may be written.
+// Any other rows, a group at a time.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ out, float* __restrict__ scales,
                                                                  int rows, int inner, int groups, long long pitch, int whole) {
-    // The successor may read what does not depend on this kernel as soon as it runs, so it is let in only when everything in front of
-    // this kernel is complete.
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31;
-    const long long warp = ((long long)blockIdx.x * kThreads + threadIdx.x) >> 5, warps = (long long)gridDim.x * (kThreads / 32);
-    const long long total = (long long)rows * groups;
-    for (long long g = warp; g < total; g += warps) {
-        const int row = (int)(g / groups), group = (int)(g - (long long)row * groups);
-        const int first = group * kGroup + 4 * lane;
-        float v[4];
-        load4(x + (size_t)row * inner, first, inner, whole != 0, v);
-        const uint32_t largest = warp_max_bits(max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3]))));
-        const Rounding r = rounding_of(largest);
-        if (first < inner) *reinterpret_cast<uint32_t*>(out + (size_t)row * pitch + first) = four_of(v[0], v[1], v[2], v[3], r.inverse);
-        if (lane == 0) scales[g] = r.scale;
+    const int place = threadIdx.x & 15;
+    const long long total = (long long)rows * groups, halves = (long long)gridDim.x * (kThreads / 16);
+    for (long long g0 = ((long long)blockIdx.x * kThreads + (threadIdx.x & ~31)) >> 4; g0 < total; g0 += halves) {
+        const long long g = g0 + ((threadIdx.x >> 4) & 1);
+        const int row = (int)(g / groups), first = (int)(g - (long long)row * groups) * kBlock + 8 * place;
+        Eight<T> numbers;
+        numbers.clear();
+        if (g < total) {
+            if (whole && first + 8 <= inner) numbers.ask(x + (size_t)row * inner + first);
+            else numbers.ask_singly(x + (size_t)row * inner, first, inner);
+        }
+        const Rounding r = rounding_of(half_warp_max(numbers.largest()));
+        if (g < total) {
+            if (first < inner) *reinterpret_cast<uint2*>(out + (size_t)row * pitch + first) = numbers.rounded(r.inverse);
+            if (place == 0) scales[g] = r.scale;
+        }
     }
 }
 
-// Block (column of blocks, row of blocks); a warp takes 16 of its 128 rows.
-template <typename T>
+// Block (column of blocks, row of blocks); a warp takes 16 of its 128 rows, two at a time.  WHOLE: rows begin at multiples of 16 bytes.
+template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) quantize_matrix_kernel(const T* __restrict__ x, unsigned char* __restrict__ out, float* __restrict__ scales,
-                                                                   int rows, int inner, int groups, long long pitch, int whole) {
+                                                                   int rows, int inner, int groups, long long pitch) {
     pdl_wait();
     pdl_trigger();
-    constexpr int kRows = kGroup / (kThreads / 32);
+    constexpr int kTurns = kBlock / (kThreads / 16);
     __shared__ uint32_t parts[kThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int first = blockIdx.x * kGroup + 4 * lane;
-    const long long row0 = (long long)blockIdx.y * kGroup + warp * kRows;
-    float v[kRows][4];
+    const int first = blockIdx.x * kBlock + 8 * (lane & 15);
+    const long long row0 = (long long)blockIdx.y * kBlock + warp * 2 * kTurns + (lane >> 4);
+    Eight<T> numbers[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+        const long long row = row0 + 2 * i;
+        if (WHOLE && row < rows && first + 8 <= inner) numbers[i].ask(x + (size_t)row * inner + first);
+        else numbers[i].clear();
+        if (!WHOLE || first + 8 > inner)
+            if (row < rows) numbers[i].ask_singly(x + (size_t)row * inner, first, inner);
+    }
     uint32_t largest = 0;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[i][c] = 0.0f;
-        if (row0 + i < rows) load4(x + (size_t)(row0 + i) * inner, first, inner, whole != 0, v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) largest = max(largest, magnitude(v[i][c]));
-    largest = warp_max_bits(largest);
+    for (int i = 0; i < kTurns; ++i) largest = max(largest, numbers[i].largest());
+    largest = __reduce_max_sync(0xffffffffu, largest);
     if (lane == 0) parts[warp] = largest;
     __syncthreads();
 #pragma unroll
@@ -92,8 +155,10 @@ __global__ void __launch_bounds__(kThreads) quantize_matrix_kernel(const T* __re
     const Rounding r = rounding_of(largest);
     if (first < inner)
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
-            if (row0 + i < rows) *reinterpret_cast<uint32_t*>(out + (size_t)(row0 + i) * pitch + first) = four_of(v[i][0], v[i][1], v[i][2], v[i][3], r.inverse);
+        for (int i = 0; i < kTurns; ++i) {
+            const long long row = row0 + 2 * i;
+            if (row < rows) *reinterpret_cast<uint2*>(out + (size_t)row * pitch + first) = numbers[i].rounded(r.inverse);
+        }
     if (threadIdx.x == 0) scales[(size_t)blockIdx.y * groups + blockIdx.x] = r.scale;
 }
 
@@ -103,27 +168,31 @@ __global__ void __launch_bounds__(kThreads) quantize_matrix_kernel(const T* __re
 // pitch a multiple of 16 and at least inner, out 16-byte aligned.
 LLM_EXPORT int llm_quantize_blocks(const void* x, int dtype, void* out, float* scales, int rows, int inner, long long pitch, int block_rows,
                                    cudaStream_t stream) {
-    if (rows < 0 || inner < 1 || pitch < inner || pitch % 16 != 0 || !aligned16(out) || (block_rows != 1 && block_rows != kGroup)) {
+    if (rows < 0 || inner < 1 || pitch < inner || pitch % 16 != 0 || !aligned16(out) || (block_rows != 1 && block_rows != kBlock)) {
         llm_set_error("quantize_blocks: %d rows of %d (pitch %lld) in blocks of %d rows", rows, inner, pitch, block_rows);
         return LLM_REFUSED;
     }
     if (rows == 0) return LLM_OK;
-    const int groups = (inner + kGroup - 1) / kGroup, row_blocks = (rows + kGroup - 1) / kGroup;
+    const int groups = (inner + kBlock - 1) / kBlock, row_blocks = (rows + kBlock - 1) / kBlock;
     if (block_rows != 1 && row_blocks > 65535) {
-        llm_set_error("quantize_blocks: at most %d rows, got %d", 65535 * kGroup, rows);
+        llm_set_error("quantize_blocks: at most %d rows, got %d", 65535 * kBlock, rows);
         return LLM_REFUSED;
     }
     LLM_DISPATCH_DTYPE(dtype, {
-        // four numbers of every row can be read at once: the rows begin at multiples of four numbers
-        const int whole = inner % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
+        const T* from = reinterpret_cast<const T*>(x);
+        unsigned char* to = reinterpret_cast<unsigned char*>(out);
+        // rows that begin at multiples of 16 bytes are read 16 bytes at a time
+        const bool whole = inner % (16 / (int)sizeof(T)) == 0 && aligned16(x);
         if (block_rows == 1) {
-            const long long warps = (long long)rows * groups, blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
+            const long long total = (long long)rows * groups, blocks = (total + kThreads / 16 - 1) / (kThreads / 16);
             const long long room = 8LL * llm_sm_count();      // blocks that run at a time
-            llm_launch(quantize_rows_kernel<T>, dim3((unsigned)(blocks < room ? blocks : room)), kThreads, 0, stream,
-                       reinterpret_cast<const T*>(x), reinterpret_cast<unsigned char*>(out), scales, rows, inner, groups, pitch, whole);
+            const dim3 grid((unsigned)(blocks < room ? blocks : room));
+            if (whole && inner % kBlock == 0 && pitch == inner) llm_launch(quantize_groups_kernel<T>, grid, kThreads, 0, stream, from, to, scales, total);
+            else llm_launch(quantize_rows_kernel<T>, grid, kThreads, 0, stream, from, to, scales, rows, inner, groups, pitch, (int)whole);
         } else {
-            llm_launch(quantize_matrix_kernel<T>, dim3(groups, row_blocks), kThreads, 0, stream, reinterpret_cast<const T*>(x),
-                       reinterpret_cast<unsigned char*>(out), scales, rows, inner, groups, pitch, whole);
+            const dim3 grid(groups, row_blocks);
+            if (whole) llm_launch(quantize_matrix_kernel<T, true>, grid, kThreads, 0, stream, from, to, scales, rows, inner, groups, pitch);
+            else llm_launch(quantize_matrix_kernel<T, false>, grid, kThreads, 0, stream, from, to, scales, rows, inner, groups, pitch);
         }
     });
     return llm_check_launch("quantize_blocks");

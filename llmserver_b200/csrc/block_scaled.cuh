@@ -29,6 +29,4 @@ __device__ __forceinline__ uint32_t four_of(float a, float b, float c, float d, 
     return (uint32_t)low | (uint32_t)high << 16;
 }
 
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }      // NaN above infinity above all others
-
 }  // namespace block_scaled
