@@ -9,10 +9,14 @@
 //
 // What a request holds is read from its history, a row of token ids of which the first `prompt` are the prompt: nothing is counted
 // from call to call, so a call that is repeated gives the same, and a request that was put out and comes back has nothing to rebuild.
-// A block takes a slice of the vocabulary of one row and keeps one word per token of the slice in shared memory: the times it stands
-// in the answer (30 bits), whether a bias is listed, whether it stands in the prompt.  It walks the row's whole history and marks the
-// tokens of its slice (integer atomics: their order does not matter), then walks the slice's logits once.  The logits of its first
-// turn are asked for before the history, so that the two reads overlap.
+// A block takes a slice of the vocabulary of one row and keeps a mark per token of the slice in shared memory: the times it stands in the
+// answer, whether a bias is listed, whether it stands in the prompt; 16 bits where histories have room for fewer than 16384 tokens, so that
+// one round of blocks holds large steps, else 32.  It walks the row's whole history and marks the tokens of its slice (integer atomics: their
+// order does not matter); whoever marks a token first puts it on a list.  The tokens of the list, a few hundred of many thousand, are worked
+// out by themselves, a token per thread.  The walk over the slice's logits then knows nothing of them: the form that returns logits
+// writes theirs over what the walk wrote, and the one that samples looks at a mark only where a logit would win.  (With the marks looked up
+// for every token the walk took twice as long, and worked out where it met them half as long again: it is bound by instructions.)  A list
+// that overflows is not used: marks are then worked out in the walk.  The slice's logits are asked into L2 before all that.
 //
 // Sampling (sampling.cu's rule) takes the controlled logits as they are made, without writing them.  A second kernel picks the best
 // slice of a row, gives -1 where nothing is left to draw from, and writes the token behind the request's history: all histories have
@@ -44,10 +48,14 @@ namespace {
 
 using Controls = LlmControls;
 
-constexpr uint32_t kPrompt = 0x80000000u, kBias = 0x40000000u, kTimes = 0x3fffffffu;
 constexpr int kThreads = 512;
+constexpr int kPerSm = 3;               // blocks that share an SM
 constexpr int kAhead = 8;               // logits a thread asks for at a time
-constexpr int kMostSlice = 13824;       // tokens per slice: 54 KiB of words, four blocks of which fit an SM
+constexpr int kIdsAhead = 8;            // ids of the history
+constexpr int kListed = 2048;           // marked tokens of a slice that are worked out by themselves
+constexpr int kMostShared = 68 << 10;   // of a block
+constexpr int kLeastSlice = 2048;       // tokens
+constexpr int kListByScan = 8 * kThreads;      // slices of so many tokens and fewer are marked first and looked through for marks afterwards
 constexpr int kBadRow = 8;              // error code: a row names a history, list or mask that does not exist
 
 // What a block needs of its row.
@@ -63,59 +71,119 @@ struct RowControls {
 };
 
 __device__ __forceinline__ RowControls controls_of(const Controls& c, int row) {
+    // asked for together, looked at afterwards
+    int at = -1, list = -1, mask = -1, length = 0, prompt = 0;
     RowControls r = {};
-    bool bad = false;
     r.repetition = 1.0f;
-    if (c.penalties != nullptr && c.history_rows != nullptr) {
+    if (c.penalties != nullptr) {
+        at = c.history_rows[row];
+        length = c.lengths[row];
+        prompt = c.prompt_lengths[row];
         r.repetition = c.penalties[3 * (size_t)row];
         r.presence = c.penalties[3 * (size_t)row + 1];
         r.frequency = c.penalties[3 * (size_t)row + 2];
-        const int at = c.history_rows[row];
-        bad |= at >= c.histories;
-        // penalties that change nothing need no history
-        if (at >= 0 && at < c.histories && (r.repetition != 1.0f || r.presence != 0.0f || r.frequency != 0.0f)) {
-            r.history = c.history + (size_t)at * c.capacity;
-            r.length = min(max(c.lengths[row], 0), c.capacity);
-            r.prompt = min(max(c.prompt_lengths[row], 0), r.length);
-        }
     }
-    if (c.bias_rows != nullptr) {
-        const int list = c.bias_rows[row];
-        bad |= list >= c.bias_lists;
-        if (list >= 0 && list < c.bias_lists) {
-            const int first = min(max(c.bias_starts[list], 0), c.bias_entries);
-            const int last = min(max(c.bias_starts[list + 1], first), c.bias_entries);
-            r.bias_ids = c.bias_ids + first;
-            r.bias_values = c.bias_values + first;
-            r.biases = last - first;
-        }
+    if (c.bias_rows != nullptr) list = c.bias_rows[row];
+    if (c.mask_rows != nullptr) mask = c.mask_rows[row];
+    if (list >= 0 && list < c.bias_lists) {
+        const int first = min(max(c.bias_starts[list], 0), c.bias_entries);
+        const int last = min(max(c.bias_starts[list + 1], first), c.bias_entries);
+        r.bias_ids = c.bias_ids + first;
+        r.bias_values = c.bias_values + first;
+        r.biases = last - first;
     }
-    if (c.mask_rows != nullptr) {
-        const int mask = c.mask_rows[row];
-        bad |= mask >= c.mask_count;
-        if (mask >= 0 && mask < c.mask_count) r.mask = c.masks + (size_t)mask * c.mask_words;
+    // penalties that change nothing need no history
+    if (at >= 0 && at < c.histories && (r.repetition != 1.0f || r.presence != 0.0f || r.frequency != 0.0f)) {
+        r.history = c.history + (size_t)at * c.capacity;
+        r.length = min(max(length, 0), c.capacity);
+        r.prompt = min(max(prompt, 0), r.length);
     }
-    if (bad && threadIdx.x == 0 && c.error_flag != nullptr) atomicExch(c.error_flag, kBadRow);
+    if (mask >= 0 && mask < c.mask_count) r.mask = c.masks + (size_t)mask * c.mask_words;
+    if (threadIdx.x == 0 && (at >= c.histories || list >= c.bias_lists || mask >= c.mask_count) && c.error_flag != nullptr) atomicExch(c.error_flag, kBadRow);
     r.marks = r.length > 0 || r.biases > 0;
     return r;
 }
 
-// Marks the tokens begin .. begin + count - 1 of the row's history and bias list.
-__device__ __forceinline__ void mark_slice(const RowControls& r, uint32_t* marks, int begin, int count) {
-    for (int i = threadIdx.x; i < count; i += blockDim.x) marks[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < r.length; i += blockDim.x) {
-        const uint32_t place = (uint32_t)r.history[i] - (uint32_t)begin;
-        if (place < (uint32_t)count) {
-            if (i < r.prompt) atomicOr(&marks[place], kPrompt);
-            else atomicAdd(&marks[place], 1u);
+// The marks of a slice: SMALL of them share a word two by two.
+template <bool SMALL>
+struct Marks {
+    static constexpr uint32_t kPrompt = SMALL ? 0x8000u : 0x80000000u, kBias = SMALL ? 0x4000u : 0x40000000u, kTimes = kBias - 1;
+    uint32_t* words;
+    static constexpr int kPerVector = SMALL ? 8 : 4;      // marks in 16 bytes
+    static __host__ __device__ int vectors_of(int count) { return (count + kPerVector - 1) / kPerVector; }
+    // Adds a flag or one more time; gives what the mark was.
+    __device__ __forceinline__ uint32_t touch(uint32_t place, uint32_t flag) const {
+        uint32_t* word = &words[SMALL ? place >> 1 : place];
+        const int shift = SMALL ? 16 * (place & 1) : 0;
+        return cut(flag ? atomicOr(word, flag << shift) : atomicAdd(word, 1u << shift), place);
+    }
+    static __device__ __forceinline__ uint32_t cut(uint32_t word, uint32_t place) { return SMALL ? word >> (16 * (place & 1)) & 0xffffu : word; }
+    __device__ __forceinline__ uint32_t of(uint32_t place) const { return cut(words[SMALL ? place >> 1 : place], place); }
+};
+
+// Marks the tokens begin .. begin + count - 1 of the row's history and bias list and lists them, each once; more than kListed are counted, and
+// only the first of them listed.  The words are zero.  Large slices list a token when it is marked first, small ones look through the
+// marks at the end: an atomic that has to answer costs more than one that has not, and a small slice belongs to a step of few rows whose
+// histories may be long.
+template <bool SMALL>
+__device__ __forceinline__ void mark_slice(const RowControls& r, Marks<SMALL> marks, uint16_t* listed, int* n_listed, int begin, int count) {
+    const bool scan = count <= kListByScan;
+    auto put = [&](int place) {
+        const int at = atomicAdd(n_listed, 1);
+        if (at < kListed) listed[at] = (uint16_t)place;
+    };
+    auto batch = [&](const int (&ids)[kIdsAhead], const uint32_t (&flags)[kIdsAhead]) {
+        if (scan) {
+#pragma unroll
+            for (int a = 0; a < kIdsAhead; ++a)
+                if ((uint32_t)ids[a] - (uint32_t)begin < (uint32_t)count) marks.touch((uint32_t)ids[a] - (uint32_t)begin, flags[a]);
+            return;
+        }
+        uint32_t before[kIdsAhead];
+#pragma unroll
+        for (int a = 0; a < kIdsAhead; ++a)
+            before[a] = (uint32_t)ids[a] - (uint32_t)begin < (uint32_t)count ? marks.touch((uint32_t)ids[a] - (uint32_t)begin, flags[a]) : 1;
+#pragma unroll
+        for (int a = 0; a < kIdsAhead; ++a)
+            if (before[a] == 0) put(ids[a] - begin);
+    };
+    // (asked for one after the other, 24 thousand ids of a row took 26 us: every turn waits for memory)
+    int next[kIdsAhead];
+    auto ask = [&](const int* from, int first, int most) {
+#pragma unroll
+        for (int a = 0; a < kIdsAhead; ++a) next[a] = first + a * kThreads < most ? from[first + a * kThreads] : -1;      // (no token: begin is not negative)
+    };
+    ask(r.history, threadIdx.x, r.length);
+    for (int first = threadIdx.x; first < r.length; first += kIdsAhead * kThreads) {
+        int ids[kIdsAhead];
+        uint32_t flags[kIdsAhead];
+#pragma unroll
+        for (int a = 0; a < kIdsAhead; ++a) {
+            ids[a] = next[a];
+            flags[a] = first + a * kThreads < r.prompt ? Marks<SMALL>::kPrompt : 0;
+        }
+        ask(r.history, first + kIdsAhead * kThreads, r.length);
+        batch(ids, flags);
+    }
+    for (int first = threadIdx.x; first < r.biases; first += kIdsAhead * kThreads) {
+        uint32_t flags[kIdsAhead];
+        ask(r.bias_ids, first, r.biases);
+#pragma unroll
+        for (int a = 0; a < kIdsAhead; ++a) flags[a] = Marks<SMALL>::kBias;
+        batch(next, flags);
+    }
+    if (scan) {
+        __syncthreads();
+        constexpr int kEach = Marks<SMALL>::kPerVector;
+        for (int v = threadIdx.x; v < Marks<SMALL>::vectors_of(count); v += kThreads) {
+            const uint4 words = reinterpret_cast<const uint4*>(marks.words)[v];
+            if ((words.x | words.y | words.z | words.w) == 0) continue;
+            const uint32_t word[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+                if (Marks<SMALL>::cut(word[SMALL ? e / 2 : e], e) != 0) put(v * kEach + e);
         }
     }
-    for (int i = threadIdx.x; i < r.biases; i += blockDim.x) {
-        const uint32_t place = (uint32_t)r.bias_ids[i] - (uint32_t)begin;
-        if (place < (uint32_t)count) atomicOr(&marks[place], kBias);
-    }
-    __syncthreads();
 }
 
 __device__ float bias_of(const RowControls& r, int token) {
@@ -129,72 +197,185 @@ __device__ float bias_of(const RowControls& r, int token) {
 }
 
 // The steps are rounded one by one (no fused multiply-add), as the formula above says.
+template <bool SMALL>
 __device__ __forceinline__ float controlled(const RowControls& r, float logit, uint32_t mark, int token) {
-    if (mark != 0) {
-        const uint32_t times = mark & kTimes;
-        if (times != 0 || (mark & kPrompt)) logit = logit > 0.0f ? __fdiv_rn(logit, r.repetition) : __fmul_rn(logit, r.repetition);
-        if (times != 0) logit = __fsub_rn(__fsub_rn(logit, __fmul_rn((float)times, r.frequency)), r.presence);
-        if (mark & kBias) logit = __fadd_rn(logit, bias_of(r, token));
-    }
+    const uint32_t times = mark & Marks<SMALL>::kTimes;
+    if (times != 0 || (mark & Marks<SMALL>::kPrompt)) logit = logit > 0.0f ? __fdiv_rn(logit, r.repetition) : __fmul_rn(logit, r.repetition);
+    if (times != 0) logit = __fsub_rn(__fsub_rn(logit, __fmul_rn((float)times, r.frequency)), r.presence);
+    if (mark & Marks<SMALL>::kBias) logit = __fadd_rn(logit, bias_of(r, token));
     return logit;
 }
 
+// A score in the order of whole numbers.
+__device__ __forceinline__ int ordered(float v) {
+    const int bits = __float_as_int(v);
+    return bits >= 0 ? bits : bits ^ 0x7fffffff;
+}
+__device__ __forceinline__ float unordered(int v) { return __int_as_float(v >= 0 ? v : v ^ 0x7fffffff); }
+
+// The draw of a row at a temperature.  Most tokens cannot win, and an upper bound of their score says so for a fifth of its price:
+// with u = 1 - v, -log u >= v, so that the noise -log(-log u) is at most -log v.  The bound's own errors (the approximate logarithm's, the
+// product's for the quotient) are below a thousandth and a millionth of the score, which it is raised by.
+struct Draw {
+    float temperature, inverse;
+    uint32_t word;      // of seed and step
+    __device__ __forceinline__ void begin(float t, uint64_t seed, uint32_t step) {
+        temperature = t;
+        inverse = 1.0f / t;
+        word = mix32(mix32(mix32((uint32_t)seed ^ 0x9E3779B9u) ^ (uint32_t)(seed >> 32)) ^ step);
+    }
+    __device__ __forceinline__ bool may_exceed(float logit, int token, float best) const {
+        const uint32_t k = mix32(word ^ (uint32_t)token) >> 9;
+        const float v = (2.0f - __uint_as_float(0x3f800000u | k)) - 1.0f / 16777216.0f;      // exact: 1 - (k + 1/2) / 2^23
+        float log2_v;
+        asm("lg2.approx.f32 %0, %1;" : "=f"(log2_v) : "f"(v));
+        const float scaled = logit * inverse;
+        return !(fmaf(-0.69314718f, log2_v, scaled) + fmaf(fabsf(scaled), 1e-6f, 1e-3f) < best);      // true where anything is a NaN
+    }
+    __device__ __forceinline__ float score(float logit, int token) const {
+        const uint32_t k = mix32(word ^ (uint32_t)token) >> 9;
+        const float u = ((float)k + 0.5f) * (1.0f / 8388608.0f);
+        const float score = logit / temperature - logf(-logf(u));
+        return score != score ? -INFINITY : score;      // a NaN never wins
+    }
+};
+
 // SAMPLE: each block leaves its slice's best score and token in `partial`; else the controlled logits go to `out` (which may be
-// `logits`).  Slices begin at multiples of 32 tokens, so that a warp's 32 tokens share a word of the mask.
-template <bool SAMPLE>
-__global__ void __launch_bounds__(kThreads) control_kernel(const float* logits, float* out, const Controls c, int vocab, int per_slice,
-                                                           const float* __restrict__ temperatures, const uint64_t* __restrict__ seeds,
-                                                           const int* __restrict__ steps, float* __restrict__ partial_scores,
-                                                           int* __restrict__ partial_indices) {
+// `logits`).  FOUR: rows begin at multiples of 16 bytes, and a thread takes four tokens side by side.
+template <bool SAMPLE, bool SMALL, bool FOUR>
+__global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* logits, float* out, const Controls c, int vocab, int per_slice,
+                                                                   const float* __restrict__ temperatures, const uint64_t* __restrict__ seeds,
+                                                                   const int* __restrict__ steps, float* __restrict__ partial_scores,
+                                                                   int* __restrict__ partial_indices) {
     pdl_trigger();
     pdl_wait();
-    extern __shared__ uint32_t marks[];
+    extern __shared__ uint4 slice_vectors[];      // the marks, then the slice of the mask
     __shared__ float best_values[kThreads / 32];
     __shared__ int best_indices[kThreads / 32];
+    __shared__ uint16_t listed[kListed];
+    __shared__ int n_listed;
+    __shared__ int bar;      // SAMPLE: a score that some token of the slice reaches
     const int row = blockIdx.y;
-    const int begin = blockIdx.x * per_slice, end = min(vocab, begin + per_slice);
+    const int begin = blockIdx.x * per_slice, end = min(vocab, begin + per_slice), count = end - begin;
     const float* src = logits + (size_t)row * vocab;
-    float values[kAhead];
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-        const int i = begin + (int)threadIdx.x + a * kThreads;
-        values[a] = i < end ? src[i] : 0.0f;
-    }
+    float* dst = out + (size_t)row * vocab;
+    if (FOUR && threadIdx.x == 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + begin), "r"(count * 4) : "memory");
     const RowControls r = controls_of(c, row);
-    if (r.marks) mark_slice(r, marks, begin, end - begin);
-    float temperature = 0.0f;
-    uint64_t seed = 0;
-    uint32_t step = 0;
-    if (SAMPLE && temperatures != nullptr) {
-        temperature = temperatures[row];
-        seed = seeds[row];
-        step = (uint32_t)steps[row];
+    const Marks<SMALL> marks{reinterpret_cast<uint32_t*>(slice_vectors)};
+    uint32_t* allowed = reinterpret_cast<uint32_t*>(slice_vectors + Marks<SMALL>::vectors_of(per_slice));
+    if (r.mask != nullptr)
+        for (int i = threadIdx.x; i < (count + 31) / 32; i += kThreads) allowed[i] = (uint32_t)r.mask[begin / 32 + i];      // (slices begin at multiples of 32)
+    if (threadIdx.x == 0) {
+        n_listed = 0;
+        bar = ordered(-INFINITY);
     }
-    float best = -INFINITY;
+    if (r.marks) {
+        for (int i = threadIdx.x; i < Marks<SMALL>::vectors_of(count); i += kThreads) slice_vectors[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        mark_slice<SMALL>(r, marks, listed, &n_listed, begin, count);
+    }
+    Draw draw = {};
+    if (SAMPLE && temperatures != nullptr && temperatures[row] > 0.0f) draw.begin(temperatures[row], seeds[row], (uint32_t)steps[row]);
+    const bool warm = draw.temperature > 0.0f;
+    __syncthreads();
+
+    // What is marked, by itself.  (Where logits are returned into their own place they are read before the walk and written behind it.)
+    const bool apart = r.marks && n_listed <= kListed, inside = r.marks && !apart;
+    float best = -INFINITY, apart_values[kListed / kThreads];
     int best_index = 0x7fffffff;
-    for (int first = begin + (int)threadIdx.x; first < end; first += kAhead * kThreads) {
-        if (first >= begin + kAhead * kThreads) {
+    if (apart) {
+#pragma unroll
+        for (int k = 0; k < kListed / kThreads; ++k) {
+            const int e = threadIdx.x + k * kThreads;
+            if (e >= n_listed) break;
+            const int place = listed[e], i = begin + place;
+            float logit = controlled<SMALL>(r, src[i], marks.of(place), i);
+            if (r.mask != nullptr && (allowed[place >> 5] >> (place & 31) & 1u) == 0) logit = -INFINITY;
+            apart_values[k] = logit;
+            if (SAMPLE && logit > -INFINITY) take_better(best, best_index, warm ? draw.score(logit, i) : logit, i);
+        }
+    }
+    constexpr int kEach = FOUR ? 4 : 1, kGroups = kAhead / kEach;      // tokens that lie side by side, groups of them
+    for (int lap = 0; lap < count; lap += kAhead * kThreads) {
+        auto place = [&](int a) { return lap + (a / kEach * kThreads + (int)threadIdx.x) * kEach + a % kEach; };
+        auto token = [&](int a) { return begin + place(a); };
+        float now[kAhead];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int i = token(g * kEach);
+            if constexpr (FOUR) {
+                const float4 v = i < end ? *reinterpret_cast<const float4*>(src + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                now[4 * g] = v.x, now[4 * g + 1] = v.y, now[4 * g + 2] = v.z, now[4 * g + 3] = v.w;
+            } else {
+                now[g] = i < end ? src[i] : -INFINITY;
+            }
+        }
+        if (inside) {
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
-                const int i = first + a * kThreads;
-                values[a] = i < end ? src[i] : 0.0f;
+                const uint32_t mark = token(a) < end ? marks.of(place(a)) : 0;
+                if (mark != 0) now[a] = controlled<SMALL>(r, now[a], mark, token(a));
             }
         }
+        if (r.mask != nullptr) {
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-            const int i = first + a * kThreads;
-            if (i >= end) break;
-            float logit = values[a];
-            if (r.marks) logit = controlled(r, logit, marks[i - begin], i);
-            if (r.mask != nullptr && ((uint32_t)__ldg(r.mask + (i >> 5)) >> (i & 31) & 1u) == 0) logit = -INFINITY;
-            if (SAMPLE) {
-                if (temperature > 0.0f) logit = logit / temperature - logf(-logf(uniform_for(seed, step, (uint32_t)i)));
-                if (logit != logit) logit = -INFINITY;      // a NaN never wins
-                take_better(best, best_index, logit, i);
-            } else {
-                out[(size_t)row * vocab + i] = logit;
+            for (int g = 0; g < kGroups; ++g) {
+                const uint32_t bits = token(g * kEach) < end ? allowed[place(g * kEach) >> 5] >> (place(g * kEach) & 31) : 0;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) now[g * kEach + e] = bits >> e & 1u ? now[g * kEach + e] : -INFINITY;
             }
         }
+        if (!SAMPLE) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const int i = token(g * kEach);
+                if (i >= end) break;
+                if constexpr (FOUR) *reinterpret_cast<float4*>(dst + i) = make_float4(now[4 * g], now[4 * g + 1], now[4 * g + 2], now[4 * g + 3]);
+                else dst[i] = now[g];
+            }
+            continue;
+        }
+        const float least = unordered(bar);      // (the first lap's is below everything)
+        auto take = [&](int a) {
+            if (apart && marks.of(place(a)) != 0) return;      // has been dealt with
+            take_better(best, best_index, warm ? draw.score(now[a], token(a)) : now[a], token(a));
+        };
+        if (warm) {
+            int from = 0;
+            if (lap == 0) {
+                // the first of each thread's logits set the bar for the others
+                if (now[0] > -INFINITY) take(0);
+                const int high = __reduce_max_sync(0xffffffffu, ordered(best));
+                if ((threadIdx.x & 31) == 0) atomicMax(&bar, high);
+                __syncthreads();
+                from = 1;
+            }
+            const float set = unordered(bar);
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+                if (a >= from && now[a] > -INFINITY && draw.may_exceed(now[a], token(a), fmaxf(best, set))) take(a);
+        } else {
+            float high = now[0];
+#pragma unroll
+            for (int a = 1; a < kAhead; ++a) high = fmaxf(high, now[a]);      // (a NaN is not)
+            // equal scores go to the lower token, whoever holds it
+            if (high >= fmaxf(best, least) && high > -INFINITY) {
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+                    if (now[a] >= best && now[a] > -INFINITY) take(a);
+            }
+            if (lap == 0) {
+                const int highest = __reduce_max_sync(0xffffffffu, ordered(best));
+                if ((threadIdx.x & 31) == 0) atomicMax(&bar, highest);
+                __syncthreads();
+            }
+        }
+    }
+    if (!SAMPLE && apart) {
+        __syncthreads();      // the walk has written what stood there
+#pragma unroll
+        for (int k = 0; k < kListed / kThreads; ++k)
+            if (threadIdx.x + k * kThreads < n_listed) dst[begin + listed[threadIdx.x + k * kThreads]] = apart_values[k];
     }
     if (!SAMPLE) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -251,21 +432,27 @@ __global__ void control_pick_kernel(const float* __restrict__ partial_scores, co
     if (row == 0) leave_flags(out + gridDim.x, flag_a, flag_b);
 }
 
-// Tokens per slice: whole waves of blocks (four share an SM), slices of at most kMostSlice and, where rows are few, of no fewer than
-// 2048 tokens.
-int slice_of(int rows, int vocab) {
-    const long long wave = 4LL * llm_sm_count();
-    int per_slice = kMostSlice;
-    for (int waves = 1; waves <= 64; ++waves) {
-        const long long slices = wave * waves / rows;
+// Whether 16 bits hold every count, and the bytes of shared memory that a slice needs.
+bool small_marks(const Controls& c) { return c.capacity <= (int)Marks<true>::kTimes; }
+size_t shared_of(int places, bool small) {
+    return (size_t)(small ? Marks<true>::vectors_of(places) : Marks<false>::vectors_of(places)) * sizeof(uint4) + places / 32 * sizeof(uint32_t);
+}
+
+// Tokens per slice, a multiple of 32: whole rounds of blocks, as few as the shared memory lets, and no fewer than kLeastSlice tokens.
+int slice_of(int rows, int vocab, bool small) {
+    const long long round = (long long)kPerSm * llm_sm_count();
+    for (long long rounds = 1;; ++rounds) {
+        const long long slices = round * rounds / rows;
         if (slices < 1) continue;
-        const long long size = (vocab + slices - 1) / slices;
-        if (size <= kMostSlice) {
-            per_slice = size < 2048 ? 2048 : (int)size;
-            break;
-        }
+        const long long each = (vocab + slices - 1) / slices;
+        if (each <= kLeastSlice) return kLeastSlice;
+        const long long size = (each + 31) / 32 * 32;
+        if (size <= 1 << 16 && shared_of((int)size, small) <= (size_t)kMostShared) return (int)size;
     }
-    return (per_slice + 31) / 32 * 32;
+}
+int slices_of(int rows, int vocab, bool small) {
+    const int size = slice_of(rows, vocab, small);
+    return (int)(((long long)vocab + size - 1) / size);
 }
 
 int refuse_controls(const char* what, const Controls& c, int rows, int vocab) {
@@ -280,30 +467,39 @@ int refuse_controls(const char* what, const Controls& c, int rows, int vocab) {
     return LLM_OK;
 }
 
-template <bool SAMPLE>
-int launch_control(const float* logits, float* out, const Controls& c, int rows, int vocab, int per_slice, const float* temperatures,
-                   const uint64_t* seeds, const int* steps, float* scores, int* indices, cudaStream_t stream) {
-    const int slices = (vocab + per_slice - 1) / per_slice;
-    const size_t shared = (size_t)(per_slice < vocab ? per_slice : vocab) * sizeof(uint32_t);
-    if (int status = llm_raise_shared_limit((const void*)control_kernel<SAMPLE>, shared, "control_logits", true)) return status;
-    llm_launch(control_kernel<SAMPLE>, dim3(slices, rows), kThreads, shared, stream, logits, out, c, vocab, per_slice, temperatures, seeds,
-               steps, scores, indices);
+template <bool SAMPLE, bool SMALL, bool FOUR>
+int launch_form(const float* logits, float* out, const Controls& c, int rows, int vocab, int per_slice, const float* temperatures,
+                const uint64_t* seeds, const int* steps, float* scores, int* indices, cudaStream_t stream) {
+    if (int status = llm_raise_shared_limit((const void*)control_kernel<SAMPLE, SMALL, FOUR>, kMostShared, "control_logits", true)) return status;
+    llm_launch(control_kernel<SAMPLE, SMALL, FOUR>, dim3((unsigned)(((long long)vocab + per_slice - 1) / per_slice), rows), kThreads,
+               shared_of(per_slice, SMALL), stream, logits, out, c, vocab, per_slice, temperatures, seeds, steps, scores, indices);
     return llm_check_launch("control_logits");
+}
+
+template <bool SAMPLE>
+int launch_control(const float* logits, float* out, const Controls& c, int rows, int vocab, const float* temperatures,
+                   const uint64_t* seeds, const int* steps, float* scores, int* indices, cudaStream_t stream) {
+    const bool small = small_marks(c), four = vocab % 4 == 0 && aligned16(logits) && (SAMPLE || aligned16(out));
+    const auto form = small ? (four ? launch_form<SAMPLE, true, true> : launch_form<SAMPLE, true, false>)
+                            : (four ? launch_form<SAMPLE, false, true> : launch_form<SAMPLE, false, false>);
+    return form(logits, out, c, rows, vocab, slice_of(rows, vocab, small), temperatures, seeds, steps, scores, indices, stream);
 }
 
 }  // namespace
 
-// How many slices a row is scanned in: the scratch of llm_control_sample holds that many scores and tokens per row.
-LLM_EXPORT int llm_control_slices(int rows, int vocab) {
+// How many slices a row is scanned in, with histories of `capacity` tokens: the scratch of llm_control_sample holds that many scores and tokens
+// per row.
+LLM_EXPORT int llm_control_slices(int rows, int vocab, int capacity) {
     if (rows < 1 || vocab < 1) return 1;
-    const int per_slice = slice_of(rows, vocab);
-    return (vocab + per_slice - 1) / per_slice;
+    Controls c = {};
+    c.capacity = capacity;
+    return slices_of(rows, vocab, small_marks(c));
 }
 
 LLM_EXPORT int llm_control_logits(const float* logits, float* out, int rows, int vocab, const LlmControls* controls, cudaStream_t stream) {
     if (int status = refuse_controls("control_logits", *controls, rows, vocab)) return status;
     if (rows == 0) return LLM_OK;
-    return launch_control<false>(logits, out, *controls, rows, vocab, slice_of(rows, vocab), nullptr, nullptr, nullptr, nullptr, nullptr, stream);
+    return launch_control<false>(logits, out, *controls, rows, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, stream);
 }
 
 // `history`: where tokens are noted, or null.  `scores` / `indices`: [rows][llm_control_slices].
@@ -312,10 +508,8 @@ LLM_EXPORT int llm_control_sample(const float* logits, const float* temperatures
                                   const int* flag_b, cudaStream_t stream) {
     if (int status = refuse_controls("sample", *controls, rows, vocab)) return status;
     if (rows == 0) return LLM_OK;
-    const int per_slice = slice_of(rows, vocab);
-    if (int status = launch_control<true>(logits, nullptr, *controls, rows, vocab, per_slice, temperatures, seeds, steps, scores, indices, stream))
-        return status;
-    llm_launch(control_pick_kernel, rows, 32, 0, stream, scores, indices, (vocab + per_slice - 1) / per_slice, out, history, *controls,
-               (int)(history != nullptr), flag_a, flag_b);
+    const int slices = slices_of(rows, vocab, small_marks(*controls));
+    if (int status = launch_control<true>(logits, nullptr, *controls, rows, vocab, temperatures, seeds, steps, scores, indices, stream)) return status;
+    llm_launch(control_pick_kernel, rows, 32, 0, stream, scores, indices, slices, out, history, *controls, (int)(history != nullptr), flag_a, flag_b);
     return llm_check_launch("control_pick");
 }

@@ -127,7 +127,7 @@ def sample_controlled(logits: torch.Tensor, temperatures, seeds, steps, out: tor
     for name, tensor, size in (("temperatures", temperatures, rows), ("seeds", seeds, rows), ("steps", steps, rows), ("tokens", out, rows + (2 if flags else 0))):
         if tensor is not None and (tensor.numel() != size or tensor.device != logits.device):
             raise KernelError(f"{rows} rows of logits on {logits.device} and {tensor.numel()} {name} on {tensor.device}")
-    slices = library().llm_control_slices(rows, vocab)
+    slices = library().llm_control_slices(rows, vocab, said.capacity)
     scratch = torch.empty((2, rows, slices), dtype=torch.float32, device=logits.device)
     call("llm_control_sample", logits.data_ptr(), pointer(temperatures), pointer(seeds), pointer(steps), out.data_ptr(), rows, vocab, ctypes.byref(said),
          controls.history.data_ptr() if note else 0, scratch.data_ptr(), scratch.data_ptr() + 4 * rows * slices,
