@@ -450,11 +450,6 @@ int slice_of(int rows, int vocab, bool small) {
         if (size <= 1 << 16 && shared_of((int)size, small) <= (size_t)kMostShared) return (int)size;
     }
 }
-int slices_of(int rows, int vocab, bool small) {
-    const int size = slice_of(rows, vocab, small);
-    return (int)(((long long)vocab + size - 1) / size);
-}
-
 int refuse_controls(const char* what, const Controls& c, int rows, int vocab) {
     if (rows < 0 || rows > 65535 || vocab < 1) {
         llm_set_error("%s: %d rows of %d logits (1 to 65535 rows per launch)", what, rows, vocab);
@@ -487,29 +482,21 @@ int launch_control(const float* logits, float* out, const Controls& c, int rows,
 
 }  // namespace
 
-// How many slices a row is scanned in, with histories of `capacity` tokens: the scratch of llm_control_sample holds that many scores and tokens
-// per row.
-LLM_EXPORT int llm_control_slices(int rows, int vocab, int capacity) {
-    if (rows < 1 || vocab < 1) return 1;
-    Controls c = {};
-    c.capacity = capacity;
-    return slices_of(rows, vocab, small_marks(c));
-}
-
 LLM_EXPORT int llm_control_logits(const float* logits, float* out, int rows, int vocab, const LlmControls* controls, cudaStream_t stream) {
     if (int status = refuse_controls("control_logits", *controls, rows, vocab)) return status;
     if (rows == 0) return LLM_OK;
     return launch_control<false>(logits, out, *controls, rows, vocab, nullptr, nullptr, nullptr, nullptr, nullptr, stream);
 }
 
-// `history`: where tokens are noted, or null.  `scores` / `indices`: [rows][llm_control_slices].
+// `history`: where tokens are noted, or null.  `scores` / `indices`: a number each for every slice of every row, of which there are at most
+// ceil(vocab / 2048).
 LLM_EXPORT int llm_control_sample(const float* logits, const float* temperatures, const uint64_t* seeds, const int* steps, int* out, int rows,
                                   int vocab, const LlmControls* controls, int* history, float* scores, int* indices, const int* flag_a,
                                   const int* flag_b, cudaStream_t stream) {
     if (int status = refuse_controls("sample", *controls, rows, vocab)) return status;
     if (rows == 0) return LLM_OK;
-    const int slices = slices_of(rows, vocab, small_marks(*controls));
+    const int per_slice = slice_of(rows, vocab, small_marks(*controls));
     if (int status = launch_control<true>(logits, nullptr, *controls, rows, vocab, temperatures, seeds, steps, scores, indices, stream)) return status;
-    llm_launch(control_pick_kernel, rows, 32, 0, stream, scores, indices, slices, out, history, *controls, (int)(history != nullptr), flag_a, flag_b);
+    llm_launch(control_pick_kernel, rows, 32, 0, stream, scores, indices, (int)(((long long)vocab + per_slice - 1) / per_slice), out, history, *controls, (int)(history != nullptr), flag_a, flag_b);
     return llm_check_launch("control_pick");
 }

@@ -176,6 +176,10 @@ def sample(logits: torch.Tensor, temperatures: Optional[torch.Tensor] = None, se
     ``controls``: the tokens are drawn from ``control_logits(logits, controls)``, which is not written; a row whose controls leave
     nothing to draw from gets -1.  ``note``: each token drawn is written behind its request's history (history[history_rows[r],
     lengths[r]], where there is room), after all rows' histories have been read."""
+    if controls is not None:
+        return sample_controlled(logits, temperatures, seeds, steps, out, flags, controls, note)
+    if note:
+        raise KernelError("tokens are noted in the history of controls, and none were given")
     check(logits, "logits", torch.float32)
     rows, vocab = logits.shape
     if temperatures is not None:
@@ -192,10 +196,6 @@ def sample(logits: torch.Tensor, temperatures: Optional[torch.Tensor] = None, se
             check(flag, "flag", torch.int32, 1)
         if out.numel() != rows + 2 or rows == 0:
             raise KernelError(f"{rows} tokens and two flags do not fit {out.numel()} elements")
-    if controls is not None:
-        return sample_controlled(logits, temperatures, seeds, steps, out, flags, controls, note)
-    if note:
-        raise KernelError("tokens are noted in the history of controls, and none were given")
     slices = library().llm_sample_slices(rows, vocab)
     scores = indices = None
     if slices > 1:      # large vocabularies are scanned by several blocks per row, merged by a second kernel

@@ -93,6 +93,16 @@ def _checked(operand: BlockScaled, block_rows: int, name: str) -> BlockScaled:
     return operand
 
 
+def _sound(operand: BlockScaled, block_rows: int) -> bool:
+    """Whether an operand is as the product takes it, in a few looks (``_checked`` says what is wrong with one that is not)."""
+    values, scales = operand.values, operand.scales
+    rows, columns = values.shape
+    stride, step = values.stride()
+    return (values.dtype is FLOAT8 and scales.dtype is torch.float32 and operand.block_rows == block_rows and step == 1 and stride % 16 == 0
+            and stride >= columns > 0 and rows > 0 and values.data_ptr() % 16 == 0 and scales.is_contiguous()
+            and scales.shape == (-(-rows // block_rows), -(-columns // BLOCK)) and scales.get_device() == values.get_device() >= 0)
+
+
 def _row_stride(values: torch.Tensor) -> int:
     """Bytes between rows; of a single row whatever the kernel may be told."""
     return values.stride(0) if values.shape[0] > 1 else _pitch(values.shape[1])
@@ -121,37 +131,40 @@ def block_linear(x, weight: BlockScaled, out: Optional[torch.Tensor] = None, out
     """y = x W^T for W in 8 bits: what ``ops.linear`` does with a ``BlockScaled`` weight.  ``x`` [N, in]: float32 or bfloat16 (brought to 8
     bits as ``quantize_blocks`` does), or a ``BlockScaled`` of single rows.  Sums and scales are 32-bit; the result is rounded once to
     ``out_dtype`` (float32 or bfloat16; default: that of ``out``, or x's, or bfloat16 where x is in 8 bits)."""
-    _checked(weight, BLOCK, "weight")
-    cols, inner = weight.values.shape
+    values = weight.values
+    if values.dim() != 2 or not _sound(weight, BLOCK):
+        _checked(weight, BLOCK, "weight")
+    cols, inner = values.shape
     quantized = isinstance(x, BlockScaled)
-    if quantized:
-        _checked(x, 1, "x")
-    else:
+    held = x.values if quantized else x
+    if not quantized:
         check(x, "x")
-        if x.dim() != 2:
-            raise KernelError(f"block_linear takes rows [N, {inner}], got {tuple(x.shape)}")
-    rows = x.shape[0]
-    if x.shape[1] != inner:
-        raise KernelError(f"x has {x.shape[1]} columns, the weight {inner}")
-    device = weight.values.device
-    if x.device != device or (out is not None and out.device != device) or weight.scales.device != device or (quantized and x.scales.device != device):
-        raise KernelError(f"the operands lie on {x.device} and {device}")
-    current_device(weight.values, "weight")
+    elif held.dim() != 2 or not _sound(x, 1):
+        _checked(x, 1, "x")
+    if held.dim() != 2:
+        raise KernelError(f"block_linear takes rows [N, {inner}], got {tuple(held.shape)}")
+    rows, columns = held.shape
+    if columns != inner:
+        raise KernelError(f"x has {columns} columns, the weight {inner}")
+    index = values.get_device()
+    if held.get_device() != index or (out is not None and out.get_device() != index):
+        raise KernelError(f"the operands lie on {held.device} and {values.device}" + ("" if out is None else f", the output on {out.device}"))
+    current_device(values, "weight")
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else torch.bfloat16 if quantized else x.dtype
-    if out_dtype not in (torch.float32, torch.bfloat16):
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
         raise KernelError(f"block_linear writes float32 or bfloat16, not {out_dtype}")
     if out is None:
-        out = torch.empty((rows, cols), dtype=out_dtype, device=device)
+        out = torch.empty((rows, cols), dtype=out_dtype, device=values.device)
     elif out.dtype != out_dtype or not out.is_contiguous() or tuple(out.shape) != (rows, cols):
         raise KernelError(f"block_linear: the output must be contiguous {out_dtype} [{rows}, {cols}], got {out.dtype} {tuple(out.shape)}")
     scratch = 0
     if quantized:
-        kind, pitch, scales, source = -1, _row_stride(x.values), x.scales.data_ptr(), x.values.data_ptr()
+        kind, pitch, scales = -1, _row_stride(held), x.scales.data_ptr()
     else:
-        kind, pitch, scales, source = dtype_code(x.dtype), _pitch(inner), 0, x.data_ptr()
-        room = torch.empty(rows * (pitch + 4 * _blocks(inner)), dtype=torch.uint8, device=device)      # the rows in 8 bits, then their scales
+        kind, pitch, scales = dtype_code(x.dtype), _pitch(inner), 0
+        room = torch.empty(rows * (pitch + 4 * _blocks(inner)), dtype=torch.uint8, device=values.device)      # the rows in 8 bits, then their scales
         scratch = room.data_ptr()
-    call("llm_block_linear", source, kind, pitch, scales, weight.values.data_ptr(), _row_stride(weight.values), weight.scales.data_ptr(),
-         out.data_ptr(), int(out_dtype == torch.float32), rows, cols, inner, scratch, wait_error_flag(device).data_ptr(), stream_handle())
+    call("llm_block_linear", held.data_ptr(), kind, pitch, scales, values.data_ptr(), _row_stride(values), weight.scales.data_ptr(), out.data_ptr(),
+         int(out_dtype is torch.float32), rows, cols, inner, scratch, wait_error_flag(values.device).data_ptr(), stream_handle())
     return out

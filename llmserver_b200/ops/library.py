@@ -28,7 +28,6 @@ SIGNATURES = {
     "llm_ssd_recurrent": [_P, _I, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _S],
     "llm_sample": [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _S],
     "llm_sample_slices": [_I, _I],
-    "llm_control_slices": [_I, _I, _I],
     "llm_control_logits": [_P, _P, _I, _I, _P, _S],
     "llm_control_sample": [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _S],
     "llm_quantize_blocks": [_P, _I, _P, _P, _I, _I, ctypes.c_longlong, _I, _S],

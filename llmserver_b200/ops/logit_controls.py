@@ -10,13 +10,13 @@ with ``controls`` draws a token from them without writing them.  Token v of a ro
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from dataclasses import dataclass
 from typing import Mapping, Optional, Sequence
 
 import torch
 
-from .library import KernelError, call, check, current_device, library, pointer, stream_handle, wait_error_flag
+from .library import KernelError, call, check, current_device, pointer, stream_handle, wait_error_flag
 
 
 @dataclass
@@ -44,14 +44,10 @@ class LogitControls:
     mask_rows: Optional[torch.Tensor] = None
 
 
-class _Controls(ctypes.Structure):      # LlmControls of csrc/logit_controls.cu
-    _fields_ = [("penalties", ctypes.c_void_p), ("history", ctypes.c_void_p), ("history_rows", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
-                ("prompt_lengths", ctypes.c_void_p), ("histories", ctypes.c_int), ("capacity", ctypes.c_int), ("bias_starts", ctypes.c_void_p),
-                ("bias_ids", ctypes.c_void_p), ("bias_values", ctypes.c_void_p), ("bias_rows", ctypes.c_void_p), ("bias_lists", ctypes.c_int),
-                ("bias_entries", ctypes.c_int), ("masks", ctypes.c_void_p), ("mask_rows", ctypes.c_void_p), ("mask_count", ctypes.c_int),
-                ("mask_words", ctypes.c_int), ("error_flag", ctypes.c_void_p)]
-
-
+# LlmControls of csrc/logit_controls.cu: penalties, history, history_rows, lengths, prompt_lengths, how many histories and how long; starts, ids,
+# values and rows of the biases, how many lists and entries; masks, mask_rows, how many masks and words; the error flag
+_DESCRIPTION = struct.Struct("@PPPPPiiPPPPiiPPiiP")
+_LEAST_SLICE = 2048        # a row is scanned in no more slices than of so many tokens
 MOST_HISTORY = (1 << 30) - 1        # tokens of a request that a 30-bit count can hold
 
 
@@ -66,44 +62,76 @@ def _checked(tensor, name: str, device: torch.device, dtype: torch.dtype, *shape
     return tensor
 
 
-def _described(logits: torch.Tensor, controls: LogitControls, note: bool = False) -> _Controls:
-    """The kernel's view of the controls, checked."""
+def _described(logits: torch.Tensor, controls: LogitControls, note: bool = False) -> bytes:
+    """The kernel's view of the controls.  Everything is looked over in one go; where something is not as it should be, ``_complaint`` says
+    what."""
     check(logits, "logits", torch.float32)
     if logits.dim() != 2:
         raise KernelError(f"logits must be [rows, vocabulary], got {tuple(logits.shape)}")
     current_device(logits, "logits")
     rows, vocab = logits.shape
+    index, whole = logits.get_device(), torch.int32
+    c = controls
+    history = lengths = prompts = history_rows = penalties = histories = capacity = 0
+    starts = ids = values = bias_rows = lists = entries = 0
+    masks = mask_rows = mask_count = words = 0
+
+    def plain(tensor, dtype, size) -> bool:
+        return tensor is not None and tensor.dtype is dtype and tensor.get_device() == index and tensor.is_contiguous() and tensor.shape == size
+
+    row = (rows,)
+    if c.history_rows is not None:
+        held = c.history
+        if (held is None or held.dtype is not whole or held.get_device() != index or not held.is_contiguous() or held.dim() != 2
+                or held.shape[1] > MOST_HISTORY or not plain(c.history_rows, whole, row) or not plain(c.lengths, whole, row)
+                or not plain(c.prompt_lengths, whole, row) or (c.penalties is not None and not plain(c.penalties, torch.float32, (rows, 3)))):
+            _complaint(logits, c)
+        history, (histories, capacity), history_rows = held.data_ptr(), held.shape, c.history_rows.data_ptr()
+        lengths, prompts = c.lengths.data_ptr(), c.prompt_lengths.data_ptr()
+        if c.penalties is not None:
+            penalties = c.penalties.data_ptr()
+    elif c.penalties is not None or note:
+        raise KernelError("penalties and noted tokens go with a history (history_rows)")
+    if c.bias_rows is not None:
+        tokens, first = c.bias_ids, c.bias_starts
+        if (tokens is None or first is None or not plain(tokens, whole, tokens.shape[:1]) or not plain(first, whole, first.shape[:1]) or first.numel() < 1
+                or not plain(c.bias_values, torch.float32, tokens.shape) or not plain(c.bias_rows, whole, row)):
+            _complaint(logits, c)
+        starts, ids, values, bias_rows = first.data_ptr(), tokens.data_ptr(), c.bias_values.data_ptr(), c.bias_rows.data_ptr()
+        lists, entries = first.numel() - 1, tokens.numel()
+    if c.mask_rows is not None:
+        bits = c.masks
+        if (bits is None or bits.dtype is not whole or bits.get_device() != index or not bits.is_contiguous() or bits.dim() != 2
+                or bits.shape[1] * 32 < vocab or not plain(c.mask_rows, whole, row)):
+            _complaint(logits, c)
+        masks, (mask_count, words), mask_rows = bits.data_ptr(), bits.shape, c.mask_rows.data_ptr()
+    return _DESCRIPTION.pack(penalties, history, history_rows, lengths, prompts, histories, capacity, starts, ids, values, bias_rows, lists, entries,
+                             masks, mask_rows, mask_count, words, wait_error_flag(logits.device).data_ptr())
+
+
+def _complaint(logits: torch.Tensor, c: LogitControls) -> None:
+    """Raises for the first tensor of the controls that is not as it should be."""
+    rows, vocab = logits.shape
     device, whole = logits.device, torch.int32
-    c, said = controls, _Controls()
     if c.history_rows is not None:
         history = _checked(c.history, "history", device, whole, None, None)
         if history.shape[1] > MOST_HISTORY:
             raise KernelError(f"a history holds at most {MOST_HISTORY} tokens, not {history.shape[1]}")
-        said.history, said.histories, said.capacity = history.data_ptr(), history.shape[0], history.shape[1]
-        said.history_rows = _checked(c.history_rows, "history_rows", device, whole, rows).data_ptr()
-        said.lengths = _checked(c.lengths, "lengths", device, whole, rows).data_ptr()
-        said.prompt_lengths = _checked(c.prompt_lengths, "prompt_lengths", device, whole, rows).data_ptr()
+        for name in ("history_rows", "lengths", "prompt_lengths"):
+            _checked(getattr(c, name), name, device, whole, rows)
         if c.penalties is not None:
-            said.penalties = _checked(c.penalties, "penalties", device, torch.float32, rows, 3).data_ptr()
-    elif c.penalties is not None or note:
-        raise KernelError("penalties and noted tokens go with a history (history_rows)")
+            _checked(c.penalties, "penalties", device, torch.float32, rows, 3)
     if c.bias_rows is not None:
-        starts = _checked(c.bias_starts, "bias_starts", device, whole, None)
-        if starts.numel() < 1:
+        if _checked(c.bias_starts, "bias_starts", device, whole, None).numel() < 1:
             raise KernelError("bias_starts holds one number more than there are lists")
         ids = _checked(c.bias_ids, "bias_ids", device, whole, None)
-        said.bias_starts, said.bias_ids = starts.data_ptr(), ids.data_ptr()
-        said.bias_values = _checked(c.bias_values, "bias_values", device, torch.float32, ids.numel()).data_ptr()
-        said.bias_rows = _checked(c.bias_rows, "bias_rows", device, whole, rows).data_ptr()
-        said.bias_lists, said.bias_entries = starts.numel() - 1, ids.numel()
+        _checked(c.bias_values, "bias_values", device, torch.float32, ids.numel())
+        _checked(c.bias_rows, "bias_rows", device, whole, rows)
     if c.mask_rows is not None:
-        masks = _checked(c.masks, "masks", device, whole, None, None)
-        if masks.shape[1] * 32 < vocab:
-            raise KernelError(f"masks of {masks.shape[1]} words do not cover {vocab} tokens")
-        said.masks, said.mask_count, said.mask_words = masks.data_ptr(), masks.shape[0], masks.shape[1]
-        said.mask_rows = _checked(c.mask_rows, "mask_rows", device, whole, rows).data_ptr()
-    said.error_flag = wait_error_flag(device).data_ptr()
-    return said
+        if _checked(c.masks, "masks", device, whole, None, None).shape[1] * 32 < vocab:
+            raise KernelError(f"masks of {c.masks.shape[1]} words do not cover {vocab} tokens")
+        _checked(c.mask_rows, "mask_rows", device, whole, rows)
+    raise KernelError("the controls do not fit the logits")
 
 
 def control_logits(logits: torch.Tensor, controls: LogitControls, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -116,21 +144,37 @@ def control_logits(logits: torch.Tensor, controls: LogitControls, out: Optional[
         if out.shape != logits.shape or out.device != logits.device:
             raise KernelError(f"the controlled logits {tuple(out.shape)} do not match {tuple(logits.shape)}")
     rows, vocab = logits.shape
-    call("llm_control_logits", logits.data_ptr(), out.data_ptr(), rows, vocab, ctypes.byref(said), stream_handle())
+    call("llm_control_logits", logits.data_ptr(), out.data_ptr(), rows, vocab, said, stream_handle())
     return out
 
 
-def sample_controlled(logits: torch.Tensor, temperatures, seeds, steps, out: torch.Tensor, flags, controls: LogitControls, note: bool) -> torch.Tensor:
-    """``ops.sample`` with controls (the types of its other arguments are checked there)."""
+def sample_controlled(logits: torch.Tensor, temperatures, seeds, steps, out: Optional[torch.Tensor], flags, controls: LogitControls, note: bool) -> torch.Tensor:
+    """``ops.sample`` with controls."""
     said = _described(logits, controls, note)
     rows, vocab = logits.shape
-    for name, tensor, size in (("temperatures", temperatures, rows), ("seeds", seeds, rows), ("steps", steps, rows), ("tokens", out, rows + (2 if flags else 0))):
-        if tensor is not None and (tensor.numel() != size or tensor.device != logits.device):
-            raise KernelError(f"{rows} rows of logits on {logits.device} and {tensor.numel()} {name} on {tensor.device}")
-    slices = library().llm_control_slices(rows, vocab, said.capacity)
-    scratch = torch.empty((2, rows, slices), dtype=torch.float32, device=logits.device)
-    call("llm_control_sample", logits.data_ptr(), pointer(temperatures), pointer(seeds), pointer(steps), out.data_ptr(), rows, vocab, ctypes.byref(said),
-         controls.history.data_ptr() if note else 0, scratch.data_ptr(), scratch.data_ptr() + 4 * rows * slices,
+    index, device = logits.get_device(), logits.device
+    if temperatures is not None:
+        for name, tensor, dtype in (("temperatures", temperatures, torch.float32), ("seeds", seeds, torch.int64), ("steps", steps, torch.int32)):
+            if tensor is None:
+                raise KernelError("temperature sampling needs seeds and steps")
+            if tensor.dtype is not dtype or tensor.get_device() != index or not tensor.is_contiguous() or tensor.numel() != rows:
+                check(tensor, name, dtype)
+                raise KernelError(f"{rows} rows of logits on {device} and {tensor.numel()} {name} on {tensor.device}")
+    if flags:
+        for flag in flags:
+            check(flag, "flag", torch.int32, 1)
+        if rows == 0:
+            raise KernelError("no tokens and two flags")
+    if out is None:
+        out = torch.empty(rows + (2 if flags else 0), dtype=torch.int32, device=device)
+    else:
+        check(out, "sampled tokens", torch.int32)
+        if out.numel() != rows + (2 if flags else 0) or out.get_device() != index:
+            raise KernelError(f"{rows} tokens{' and two flags' if flags else ''} do not fit {out.numel()} elements on {out.device}")
+    most = rows * -(-vocab // _LEAST_SLICE)       # a score and a token for each slice of each row
+    scratch = torch.empty(2 * most, dtype=torch.float32, device=device)
+    call("llm_control_sample", logits.data_ptr(), pointer(temperatures), pointer(seeds), pointer(steps), out.data_ptr(), rows, vocab, said,
+         controls.history.data_ptr() if note else 0, scratch.data_ptr(), scratch.data_ptr() + 4 * most,
          *((flags[0].data_ptr(), flags[1].data_ptr()) if flags else (0, 0)), stream_handle())
     return out
 

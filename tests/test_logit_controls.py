@@ -1,12 +1,10 @@
 """The host's side of controls on logits: lists and masks from what a request says, and what is refused before a launch."""
-import ctypes
-
 import pytest
 import torch
 
 from llmserver_b200 import ops
 from llmserver_b200.ops import KernelError
-from llmserver_b200.ops.logit_controls import _Controls
+from llmserver_b200.ops.logit_controls import _DESCRIPTION
 
 
 def test_lists_ascend_and_stay_apart():
@@ -40,10 +38,10 @@ def test_logits_on_the_host_are_refused():
 
 def test_the_launchers_refuse_sizes_they_cannot_take():
     library = ops.library()
-    said = _Controls()
+    said = _DESCRIPTION.pack(*[0] * 18)
     for rows, vocab in ((-1, 5), (65536, 5), (1, 0)):
-        assert library.llm_control_logits(0, 0, rows, vocab, ctypes.byref(said), 0) == -1
-        assert library.llm_control_sample(0, 0, 0, 0, 0, rows, vocab, ctypes.byref(said), 0, 0, 0, 0, 0, 0) == -1
-    said.masks, said.mask_words = 16, 3
-    assert library.llm_control_logits(0, 0, 1, 97, ctypes.byref(said), 0) == -1 and b"words" in library.llm_last_error()
-    assert library.llm_control_logits(0, 0, 0, 96, ctypes.byref(said), 0) == 0
+        assert library.llm_control_logits(0, 0, rows, vocab, said, 0) == -1
+        assert library.llm_control_sample(0, 0, 0, 0, 0, rows, vocab, said, 0, 0, 0, 0, 0, 0) == -1
+    said = _DESCRIPTION.pack(*[0] * 13, 16, 0, 1, 3, 0)
+    assert library.llm_control_logits(0, 0, 1, 97, said, 0) == -1 and b"words" in library.llm_last_error()
+    assert library.llm_control_logits(0, 0, 0, 96, said, 0) == 0
