@@ -2,7 +2,8 @@
 
     python -m llmserver_b200.cli.generate --model DIR --prompt-ids 1,2,3 [--prompt-ids 7,8 ...]
            [--max-new-tokens 32] [--temperature 0.0] [--seed 0] [--ignore-eos] [--dtype bfloat16]
-           [--block-size 16] [--max-batch-size 8] [--max-num-batched-tokens 8192] [--json]
+           [--block-size 16] [--max-batch-size 8] [--max-num-batched-tokens 8192] [--json] [--products float8]
+           [--repetition-penalty 1.0] [--presence-penalty 0.0] [--frequency-penalty 0.0] [--logit-bias 17=-100 ...]
     python -m llmserver_b200.cli.generate --random-config config.json --seed 0 --prompt-ids ...
 
 The engine works on token ids (it has no tokenizer), so prompts are comma-separated ids, one ``--prompt-ids`` per
@@ -28,6 +29,14 @@ def _ids(text: str):
         raise argparse.ArgumentTypeError(f"token ids are integers separated by commas: {error}") from error
 
 
+def _bias(text: str):
+    try:
+        token, value = text.split("=")
+        return int(token), float(value)
+    except ValueError as error:
+        raise argparse.ArgumentTypeError(f"a bias is written TOKEN=VALUE: {error}") from error
+
+
 def main(argv=None) -> int:
     parser = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     parser.add_argument("--model", help="folder with config.json and model.safetensors")
@@ -37,6 +46,11 @@ def main(argv=None) -> int:
     parser.add_argument("--max-new-tokens", type=int, default=32)
     parser.add_argument("--temperature", type=float, default=0.0)
     parser.add_argument("--seed", type=int, default=0, help="seed of the weights (--random-config) and of the sampler; request i samples with seed + i")
+    parser.add_argument("--repetition-penalty", type=float, default=1.0)
+    parser.add_argument("--presence-penalty", type=float, default=0.0)
+    parser.add_argument("--frequency-penalty", type=float, default=0.0)
+    parser.add_argument("--logit-bias", type=_bias, action="append", default=[], metavar="TOKEN=VALUE", help="added to the token's logit")
+    parser.add_argument("--products", default="same", choices=["same", "float8"], help="in what feed-forward and head matrices are held")
     parser.add_argument("--ignore-eos", action="store_true")
     parser.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     parser.add_argument("--device", default="cuda:0")
@@ -61,16 +75,18 @@ def main(argv=None) -> int:
     from ..models import load_model, random_model
 
     if args.model:
-        model = load_model(args.model, args.dtype, args.device)
+        model = load_model(args.model, args.dtype, args.device, args.products)
     else:
         with open(args.random_config) as handle:
             raw = json.load(handle)
-        model = random_model(architecture_of(raw).config_class.from_dict(raw), args.seed, args.dtype, args.device)
+        model = random_model(architecture_of(raw).config_class.from_dict(raw), args.seed, args.dtype, args.device, products=args.products)
     longest = max(len(prompt) for prompt in prompts) + args.max_new_tokens
     engine = Engine(model, max_new_tokens=args.max_new_tokens, max_batch_size=args.max_batch_size,
                     max_num_batched_tokens=args.max_num_batched_tokens, kv_cache_block_size=args.block_size,
                     ignore_eos=args.ignore_eos, cuda_graphs=not args.no_cuda_graphs, max_context=longest)
-    requests = [engine.add_request(prompt_token_ids=prompt, temperature=args.temperature, seed=args.seed + index)
+    requests = [engine.add_request(prompt_token_ids=prompt, temperature=args.temperature, seed=args.seed + index,
+                                   repetition_penalty=args.repetition_penalty, presence_penalty=args.presence_penalty,
+                                   frequency_penalty=args.frequency_penalty, logit_bias=dict(args.logit_bias))
                 for index, prompt in enumerate(prompts)]
     while engine.step():
         pass

@@ -24,7 +24,7 @@ from typing import Dict, Iterable, List, Optional, Sequence
 import torch
 
 from ..cache import CacheManager, KVCacheExhaustedError
-from ..sampling import Sampler, SamplingRow
+from ..sampling import RequestControls, Sampler, SamplingRow
 from .request import Request, RequestFinishReason, RequestStatus
 from .scheduler import PageBudget, Scheduler, StepPlan
 from .step import StepFunction
@@ -36,14 +36,17 @@ class Engine:
                  kv_cache_block_size: int = 16, ignore_eos: bool = False, cuda_graphs: Optional[bool] = None,
                  prefix_caching: bool = True, eos_token_ids: Optional[Iterable[int]] = None, dtype="bfloat16",
                  device="cuda:0", max_context: Optional[int] = None, cache: Optional[CacheManager] = None,
-                 step_function: Optional[StepFunction] = None, sampler=None):
-        """``model``: a model folder (config.json + model.safetensors) or a loaded ``DecoderModel``.
+                 step_function: Optional[StepFunction] = None, sampler=None, products: str = "same"):
+        """``model``: a model folder (config.json + model.safetensors) or a loaded ``DecoderModel``.  ``products`` ("same" or "float8"): in
+        what a folder's feed-forward and head matrices are held (``parts.Runtime``); a loaded model has been told already.
 
         ``kv_cache_num_blocks`` defaults to the reference benchmark's sizing rule
         (benchmark_cuda.py:107-111): max_batch_size * ceil(max_context / block_size) + 8 pages."""
         if isinstance(model, str):
             from ..models import load_model
-            model = load_model(model, dtype, device)
+            model = load_model(model, dtype, device, products)
+        elif products not in ("same", model.runtime.products):
+            raise ValueError(f"the model was loaded with products {model.runtime.products!r}, not {products!r}")
         if max_new_tokens <= 0:
             raise ValueError(f"max_new_tokens is <= 0: {max_new_tokens}")
         self.model = model
@@ -85,8 +88,10 @@ class Engine:
     # ------------------------------------------------------------------ requests
     def add_request(self, prompt=None, prompt_token_ids: Optional[Sequence[int]] = None,
                     max_new_tokens: Optional[int] = None, temperature: float = 0.0, seed: Optional[int] = None,
-                    ignore_eos: Optional[bool] = None) -> Request:
-        """Queues a request.  ``prompt`` exists for signature parity with the reference
+                    ignore_eos: Optional[bool] = None, **controls) -> Request:
+        """Queues a request.  ``controls``: ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` and
+        ``allowed_tokens`` (see ``sampling.RequestControls``); a request whose controls leave no token to draw ends with the reason
+        "error".  ``prompt`` exists for signature parity with the reference
         (utils/engine.py:210) and must be None or a sequence of ids: text needs a tokenizer, which
         this engine does not have."""
         if prompt_token_ids is None:
@@ -104,9 +109,11 @@ class Engine:
         budget = max_new_tokens or self.max_new_tokens
         if limit is not None and len(prompt_token_ids) + budget > limit + 1:
             raise ValueError(f"prompt of {len(prompt_token_ids)} tokens plus {budget} new tokens exceeds max_position_embeddings {limit}")
+        steering = RequestControls(**controls).check(vocab)
         index = next(self._ids)
         request = Request(f"req-{index}", prompt_token_ids, budget, temperature,
-                          seed if seed is not None else index, self.ignore_eos if ignore_eos is None else ignore_eos)
+                          seed if seed is not None else index, self.ignore_eos if ignore_eos is None else ignore_eos,
+                          steering if steering.active else None)
         self.active_requests[request.request_id] = request
         self.scheduler.waiting.append(request)
         return request
@@ -196,7 +203,8 @@ class Engine:
             entries.append((request.request_id, request.feed[first:first + share.tokens], [share.tokens - 1] if wants else []))
             if wants:
                 sampled.append(request)
-        rows = [SamplingRow(request.temperature, request.seed, len(request.generated_token_ids)) for request in sampled]
+        rows = [SamplingRow(request.temperature, request.seed, len(request.generated_token_ids), request if request.controls is not None else None)
+                for request in sampled]
         if self.record_steps:
             held = [(share.request.num_computed_tokens, share.tokens) for share in plan.shares]
             self.step_log.append((len(plan.decoding), sum(share.tokens for share in plan.prompts), len(sampled),
@@ -239,6 +247,11 @@ class Engine:
                 for name in ("schedule_s", "pack_copy_s", "launch_s", "read_back_s", "accept_s", "step_s")}
 
     def _accept(self, request: Request, token: int) -> None:
+        if token < 0:      # its controls left nothing to draw from
+            request.finish(RequestFinishReason.ERROR)
+            self._release(request)
+            self._archive(request)
+            return
         request.take(token)
         self.stats["tokens"] += 1
         if token in self.eos_token_ids and not request.ignore_eos:
@@ -262,10 +275,11 @@ class Engine:
 
     # ------------------------------------------------------------------ convenience
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: Optional[int] = None, temperature: float = 0.0,
-                 seed: Optional[int] = None, ignore_eos: Optional[bool] = None) -> List[List[int]]:
-        """Runs the given prompts (lists of token ids) to completion; returns the generated ids."""
+                 seed: Optional[int] = None, ignore_eos: Optional[bool] = None, **controls) -> List[List[int]]:
+        """Runs the given prompts (lists of token ids) to completion; returns the generated ids.  ``controls`` as in ``add_request``, the
+        same for every prompt."""
         requests = [self.add_request(prompt_token_ids=prompt, max_new_tokens=max_new_tokens, temperature=temperature,
-                                     seed=None if seed is None else seed + index, ignore_eos=ignore_eos)
+                                     seed=None if seed is None else seed + index, ignore_eos=ignore_eos, **controls)
                     for index, prompt in enumerate(prompts)]
         while self.step():
             pass

@@ -42,7 +42,7 @@ _OVER = (RequestStatus.FINISHED, RequestStatus.CANCELLED)
 
 class Request:
     def __init__(self, request_id: str, prompt_token_ids: List[int], max_new_tokens: int, temperature: float = 0.0,
-                 seed: int = 0, ignore_eos: bool = False):
+                 seed: int = 0, ignore_eos: bool = False, controls=None):
         if len(prompt_token_ids) == 0:
             raise ValueError(f"request {request_id!r} has an empty prompt")
         if max_new_tokens < 1:
@@ -54,6 +54,7 @@ class Request:
         self.generated_token_ids: List[int] = []
         self.max_new_tokens = max_new_tokens
         self.temperature, self.seed, self.ignore_eos = float(temperature), int(seed), ignore_eos
+        self.controls = controls          # sampling.RequestControls, or None
         self.status = RequestStatus.WAITING
         self.finish_reason: Optional[RequestFinishReason] = None
         self.num_computed_tokens = 0      # tokens of ``feed`` whose keys and values are in the cache

@@ -16,7 +16,7 @@ import torch
 from .. import ops
 from ..cache import CacheManager, KVCacheExhaustedError
 from ..ops.library import check_wait_errors, wait_error_flag
-from ..sampling import Sampler, SamplingRow
+from ..sampling import ControlTable, Sampler, SamplingRow
 from .batch import SequenceSlice, StepBatch, build_batch
 
 StepEntry = Tuple[object, Sequence[int], Sequence[int]]  # (request id, next tokens, wanted places)
@@ -34,6 +34,7 @@ class StepFunction:
         self.graphs = None
         self.graph_steps = 0
         self.sampler = Sampler(self.device)
+        self.controls: Optional[ControlTable] = None      # made when the first request with controls is sampled
         self.last_phases = {"pack_copy": 0.0, "launch": 0.0, "read_back": 0.0}
 
     # ------------------------------------------------------------------ request lifetime
@@ -48,6 +49,8 @@ class StepFunction:
     def release(self, request_id) -> None:
         self.cache.free(request_id)
         del self.computed[request_id]
+        if self.controls is not None:
+            self.controls.forget(request_id)
         if self.graphs is not None:
             self.graphs.forget_rows()
 
@@ -120,9 +123,14 @@ class StepFunction:
 
     def run_and_sample(self, entries: List[StepEntry], sampling: Sequence, sampler=None) -> List[int]:
         """Runs one step and samples one token per wanted place (``sampling``: one row per wanted place
-        with ``temperature``, ``seed``, ``step``).  Returns the tokens on the host: the step's only
+        with ``temperature``, ``seed``, ``step`` and, where the request has controls, ``request``).  Returns the tokens on the host: the step's only
         device-to-host read, which also brings the kernels' error flag.  ``last_phases`` then holds the host
         seconds of the step's phases: ``pack_copy``, ``launch``, ``read_back``."""
+        steered = [getattr(row, "request", None) for row in sampling]
+        if not any(request is not None for request in steered):
+            steered = None
+        elif not hasattr(sampler or self.sampler, "steered_from_batch"):
+            raise ValueError("a sampler of the caller's own does not know requests' controls")
         if sampler is not None and not hasattr(sampler, "from_batch"):
             logits = self.run(entries)       # a sampler of the caller's own (tests use one on the CPU)
             return sampler(logits, sampling) if sampling else []
@@ -138,8 +146,21 @@ class StepFunction:
                 advanced = True
                 self._advance(entries)
 
+        described = None
+
+        def describe() -> None:     # before anything moves on: a grammar of the caller's may raise
+            nonlocal described
+            if steered is not None:
+                if self.controls is None:
+                    self.controls = ControlTable(self.device, self.model.spec.vocab_size)
+                described = self.controls.describe(steered)
+
+        def meanwhile() -> None:
+            describe()
+            advance()
+
         if graph is not None:
-            graph.meanwhile = advance
+            graph.meanwhile = meanwhile
             try:
                 result = graph.run(slices, sampling, self.last_phases)
             finally:
@@ -147,6 +168,13 @@ class StepFunction:
             self.last_phases["pack_copy"] += graph.began - began
             self.last_batch_bytes = graph.layout.total * 4
             self.graph_steps += 1
+            if steered is not None:
+                # the graph has drawn without controls; its logits are still there
+                began = clock()
+                tokens = (sampler or self.sampler).steered_from_batch(graph.logits[:len(slices)], graph.batch, described)
+                flags = torch.cat([tokens, wait_error_flag(self.device)]).tolist()
+                result = flags[:-1] + [result[-2], flags[-1]]
+                self.last_phases["read_back"] += clock() - began
         else:
             batch = build_batch(slices, len(self.cache.groups), self.device, self.model.spec.vocab_size, sampling=sampling)
             packed = clock()
@@ -158,7 +186,11 @@ class StepFunction:
                 self._advance(entries)
                 self.last_phases.update(pack_copy=packed - began, launch=clock() - packed, read_back=0.0)
                 return []
-            tokens = (sampler or self.sampler).from_batch(logits, batch)
+            describe()
+            if steered is not None:
+                tokens = (sampler or self.sampler).steered_from_batch(logits, batch, described)
+            else:
+                tokens = (sampler or self.sampler).from_batch(logits, batch)
             flags = torch.cat([tokens, batch.error_flag, wait_error_flag(self.device)])
             launched = clock()
             advance()

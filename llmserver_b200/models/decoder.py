@@ -49,6 +49,8 @@ class DecoderModel:
                                     for local in norm_cls.declare_weights(spec.final_norm.as_dict())}, runtime)
         # tied head: the same tensor as the embedding (utils/model_loader.py:56-57)
         self.head = self.embedding if spec.tie_head else source.get(spec.head_name).contiguous()
+        if runtime.products == "float8":
+            self.head = ops.quantize_blocks(self.head, 128)
         self.entry_caches: Optional[List[EntryCache]] = None
 
     # ------------------------------------------------------------------ cache

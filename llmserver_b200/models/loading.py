@@ -24,13 +24,13 @@ def as_dtype(dtype) -> torch.dtype:
     return DTYPES[dtype]
 
 
-def load_model(model_dir: str, dtype="bfloat16", device="cuda:0") -> DecoderModel:
+def load_model(model_dir: str, dtype="bfloat16", device="cuda:0", products: str = "same") -> DecoderModel:
     """Reads config.json, chooses the model by its architecture name and loads model.safetensors.
     The reference's ``model_loader`` (utils/model_loader.py:18-86) does the same through a Hugging
-    Face module tree; only local folders are read here."""
+    Face module tree; only local folders are read here.  ``products``: see ``parts.Runtime``."""
     config, architecture = read_config(model_dir)
     spec = architecture.build_spec(config)
-    runtime = Runtime(as_dtype(dtype), torch.device(device))
+    runtime = Runtime(as_dtype(dtype), torch.device(device), products)
     eos = generation_eos_ids(model_dir)
     if eos is not None:
         spec.eos_token_ids = eos
@@ -52,11 +52,11 @@ def generation_eos_ids(model_dir: str):
     return (int(eos),) if isinstance(eos, int) else tuple(int(token) for token in eos)
 
 
-def random_model(config, seed: int, dtype="bfloat16", device="cuda:0", spec=None) -> DecoderModel:
+def random_model(config, seed: int, dtype="bfloat16", device="cuda:0", spec=None, products: str = "same") -> DecoderModel:
     """A model with seeded random weights made on the device (nothing is written or read)."""
     if spec is None:
         spec = ARCHITECTURES[config.architecture].build_spec(config)
-    runtime = Runtime(as_dtype(dtype), torch.device(device))
+    runtime = Runtime(as_dtype(dtype), torch.device(device), products)
     model = DecoderModel(spec, RandomSource(spec, seed, runtime.dtype, runtime.device), runtime)
     model.config = config
     return model

@@ -144,8 +144,8 @@ def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor, group: int = GATE_U
 def gate_up_silu(x, weight: torch.Tensor, group: int = 0) -> torch.Tensor:
     """silu(x Wg^T) * (x Wu^T) for the fused weight ``weight`` [2 I, H] (halves when ``group`` is 0, else interleaved in
     groups): as one kernel where the product kernel can apply the gate in its epilogue (bfloat16, groups of 64, few
-    rows), else as the product followed by ``silu_mul``.  ``x`` may be a ``RowScaled``."""
-    if x.dtype == torch.bfloat16 and group == GATE_UP_GROUP:
+    rows), else as the product followed by ``silu_mul`` (so with a ``BlockScaled`` weight).  ``x`` may be a ``RowScaled``."""
+    if x.dtype == torch.bfloat16 and group == GATE_UP_GROUP and not isinstance(weight, BlockScaled):
         from . import gemm_bf16
         fused = gemm_bf16.gate_up_silu_fused(x, weight)
         if fused is None and x.shape[0] >= gemm_bf16.PAIR_MIN_ROWS:
@@ -1386,6 +1386,8 @@ def linear(x, weight: torch.Tensor, out: Optional[torch.Tensor] = None,
     if x.device.type != "cuda":
         raise KernelError("linear: there is no CPU path")
     if isinstance(weight, BlockScaled):
+        if isinstance(x, RowScaled):
+            raise KernelError("linear: a weight in 8 bits takes rows that have been divided by their root mean square")
         return block_linear(x, weight, out=out, out_dtype=out_dtype)
     if x.dtype == torch.float32:
         result = gemm_f32(x, weight, out, settled=True)
@@ -1409,7 +1411,9 @@ def linear_wide(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
 
 
 def unscaled_rows_supported(weight: torch.Tensor) -> bool:
-    """Whether products with ``weight`` take ``RowScaled`` rows."""
+    """Whether products with ``weight`` take ``RowScaled`` rows (those with a ``BlockScaled`` weight do not)."""
+    if isinstance(weight, BlockScaled):
+        return False
     from . import gemm_bf16
     return gemm_bf16.unscaled_rows_supported(weight)
 

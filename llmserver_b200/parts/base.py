@@ -25,8 +25,15 @@ from ..weights.declare import WeightDecl
 
 @dataclass
 class Runtime:
+    """``products``: in what the matrices of dense SiLU-gated feed-forwards and of the output head are held; "same" (the dtype) or
+    "float8" (8 bits with a scale for each 128 x 128, their inputs brought to 8 bits row by row)."""
     dtype: torch.dtype
     device: torch.device
+    products: str = "same"
+
+    def __post_init__(self):
+        if self.products not in ("same", "float8"):
+            raise ValueError(f"products are held as \"same\" or \"float8\", not {self.products!r}")
 
 
 class Part:

@@ -15,7 +15,8 @@ from .registry import FEED_FORWARDS
 class SwiGLU(FeedForward):
     """down(silu(gate(x)) * up(x)) without biases (utils/layers.py:182-218).  gate and up are
     concatenated once at load into one [2 I, H] matrix, gate rows first, as the reference's
-    ``fuse_projections`` (utils/layers.py:194-203).  Parameters: ``hidden``, ``intermediate``; ``bias`` must be off
+    ``fuse_projections`` (utils/layers.py:194-203).  Where the runtime holds products in 8 bits both matrices are brought there once, here,
+    and steps run the plain product and activation kernels.  Parameters: ``hidden``, ``intermediate``; ``bias`` must be off
     and ``activation``, if given, "silu"."""
 
     KNOWN_PARAMS = ("hidden", "intermediate", "bias", "activation")
@@ -40,9 +41,12 @@ class SwiGLU(FeedForward):
         gate, up = weights["gate_proj.weight"], weights["up_proj.weight"]
         # bfloat16: gate and up rows interleaved in groups of 64, the layout in which the product kernel for few rows
         # can apply the gate itself; the 32-bit path keeps gate rows first
-        self.group = ops.GATE_UP_GROUP if gate.dtype == torch.bfloat16 and gate.shape[0] % ops.GATE_UP_GROUP == 0 else 0
+        eight_bits = runtime.products == "float8"
+        self.group = ops.GATE_UP_GROUP if gate.dtype == torch.bfloat16 and gate.shape[0] % ops.GATE_UP_GROUP == 0 and not eight_bits else 0
         self.gate_up = ops.interleave_gate_up(gate, up) if self.group else torch.cat([gate, up], dim=0).contiguous()
         self.down = weights["down_proj.weight"].contiguous()
+        if eight_bits:
+            self.gate_up, self.down = ops.quantize_blocks(self.gate_up, 128), ops.quantize_blocks(self.down, 128)
 
     feeds_stream = True
 

@@ -1,3 +1,4 @@
+from .controls import ControlTable, RequestControls
 from .sampler import Sampler, SamplingRow
 
-__all__ = ["Sampler", "SamplingRow"]
+__all__ = ["ControlTable", "RequestControls", "Sampler", "SamplingRow"]

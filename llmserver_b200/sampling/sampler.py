@@ -22,6 +22,7 @@ class SamplingRow:
     temperature: float = 0.0
     seed: int = 0
     step: int = 0     # how many tokens the request has generated before this one
+    request: object = None     # the request itself, where it has controls (``sampling.controls``)
 
 
 class Sampler:
@@ -39,6 +40,13 @@ class Sampler:
         """Samples with the per-row inputs that crossed to the device inside the step's batch; the tokens
         stay on the device (the step function reads them back together with its error flags)."""
         return ops.sample(logits, batch.temperatures, batch.seeds, batch.sample_steps)
+
+    def steered_from_batch(self, logits: torch.Tensor, batch, controls) -> torch.Tensor:
+        """``from_batch`` under the rows' controls; each token drawn is noted in its request's history, and a row whose controls leave
+        nothing to draw from gets -1.  ``batch`` may have more rows than there are logits (a padded decode step)."""
+        rows = logits.shape[0]
+        return ops.sample(logits, batch.temperatures[:rows], batch.seeds[:rows], batch.sample_steps[:rows], controls=controls,
+                          note=controls.history_rows is not None)
 
     def sample_on_device(self, logits: torch.Tensor, rows: Sequence[SamplingRow]) -> torch.Tensor:
         if any(row.temperature > 0 for row in rows):
