@@ -16,7 +16,7 @@
 // out by themselves, a token per thread.  The walk over the slice's logits then knows nothing of them: the form that returns logits
 // writes theirs over what the walk wrote, and the one that samples looks at a mark only where a logit would win.  (With the marks looked up
 // for every token the walk took twice as long, and worked out where it met them half as long again: it is bound by instructions.)  A list
-// that overflows is not used: marks are then worked out in the walk.  The slice's logits are asked into L2 before all that.
+// that overflows is not used: marks are then worked out in the walk.
 //
 // Sampling (sampling.cu's rule) takes the controlled logits as they are made, without writing them.  A second kernel picks the best
 // slice of a row, gives -1 where nothing is left to draw from, and writes the token behind the request's history: all histories have
@@ -259,7 +259,6 @@ __global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* 
     const int begin = blockIdx.x * per_slice, end = min(vocab, begin + per_slice), count = end - begin;
     const float* src = logits + (size_t)row * vocab;
     float* dst = out + (size_t)row * vocab;
-    if (FOUR && threadIdx.x == 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + begin), "r"(count * 4) : "memory");
     const RowControls r = controls_of(c, row);
     const Marks<SMALL> marks{reinterpret_cast<uint32_t*>(slice_vectors)};
     uint32_t* allowed = reinterpret_cast<uint32_t*>(slice_vectors + Marks<SMALL>::vectors_of(per_slice));
@@ -279,20 +278,17 @@ __global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* 
     const bool warm = draw.temperature > 0.0f;
     __syncthreads();
 
-    // What is marked, by itself.  (Where logits are returned into their own place they are read before the walk and written behind it.)
-    const bool apart = r.marks && n_listed <= kListed, inside = r.marks && !apart;
-    float best = -INFINITY, apart_values[kListed / kThreads];
+    const bool apart = r.marks && n_listed <= kListed, inside = r.marks && !apart;      // where what is marked is worked out
+    float best = -INFINITY, listed_logits[SAMPLE ? 1 : kListed / kThreads];
     int best_index = 0x7fffffff;
-    if (apart) {
+    // Logits that are returned into their own place are read before the walk writes there; others behind it, from L2: in front of it they waited
+    // for memory behind the walks of other blocks.
+    const bool in_place = !SAMPLE && logits == out;
+    if (apart && in_place) {
 #pragma unroll
         for (int k = 0; k < kListed / kThreads; ++k) {
             const int e = threadIdx.x + k * kThreads;
-            if (e >= n_listed) break;
-            const int place = listed[e], i = begin + place;
-            float logit = controlled<SMALL>(r, src[i], marks.of(place), i);
-            if (r.mask != nullptr && (allowed[place >> 5] >> (place & 31) & 1u) == 0) logit = -INFINITY;
-            apart_values[k] = logit;
-            if (SAMPLE && logit > -INFINITY) take_better(best, best_index, warm ? draw.score(logit, i) : logit, i);
+            listed_logits[SAMPLE ? 0 : k] = e < n_listed ? src[begin + listed[e]] : 0.0f;
         }
     }
     constexpr int kEach = FOUR ? 4 : 1, kGroups = kAhead / kEach;      // tokens that lie side by side, groups of them
@@ -371,11 +367,18 @@ __global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* 
             }
         }
     }
-    if (!SAMPLE && apart) {
-        __syncthreads();      // the walk has written what stood there
+    if (apart) {
+        if (!SAMPLE) __syncthreads();      // the walk has written what stood there
 #pragma unroll
-        for (int k = 0; k < kListed / kThreads; ++k)
-            if (threadIdx.x + k * kThreads < n_listed) dst[begin + listed[threadIdx.x + k * kThreads]] = apart_values[k];
+        for (int k = 0; k < kListed / kThreads; ++k) {
+            const int e = threadIdx.x + k * kThreads;
+            if (e >= n_listed) break;
+            const int place = listed[e], i = begin + place;
+            float logit = controlled<SMALL>(r, in_place ? listed_logits[SAMPLE ? 0 : k] : src[i], marks.of(place), i);
+            if (r.mask != nullptr && (allowed[place >> 5] >> (i & 31) & 1u) == 0) logit = -INFINITY;
+            if (!SAMPLE) dst[i] = logit;
+            else if (logit > -INFINITY) take_better(best, best_index, warm ? draw.score(logit, i) : logit, i);
+        }
     }
     if (!SAMPLE) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
