@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* 
     __shared__ int best_indices[kThreads / 32];
     __shared__ uint16_t listed[kListed];
     __shared__ int n_listed;
-    __shared__ int bar;      // SAMPLE: a score that some token of the slice reaches
+    __shared__ int bar;      // SAMPLE: a score that some token of the slice reaches; raised as the walk goes on (left at the first lap's, 64 rows took 32 us and not 30)
     const int row = blockIdx.y;
     const int begin = blockIdx.x * per_slice, end = min(vocab, begin + per_slice), count = end - begin;
     const float* src = logits + (size_t)row * vocab;
@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* 
 #pragma unroll
             for (int a = 0; a < kAhead; ++a)
                 if (a >= from && now[a] > -INFINITY && draw.may_exceed(now[a], token(a), fmaxf(best, set))) take(a);
+            if (best > set) atomicMax(&bar, ordered(best));      // for everybody's next laps
         } else {
             float high = now[0];
 #pragma unroll
