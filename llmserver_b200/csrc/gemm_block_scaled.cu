@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
             buffer.step(kBuffers);
         }
         if (!ok) failed = 1;
-        } else if (warp == 2) {
+    } else if (warp == 2) {
         // A lane's tokens' scales times W's, asked for kScalesAhead units before.
         constexpr int kMine = TOKENS < 32 ? 1 : TOKENS / 32;
         const float* w_scales = p.w_scales + (size_t)tile * p.groups + first;
@@ -248,6 +248,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     tc5::fence_after();
     if (failed)      // a wait ran out: copies that may still be in flight get time to land
         for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    // given back in front of the cluster's barriers: a block that holds tensor memory waits for nobody who may be waiting for some
+    if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns));
     if (p.split > 1) {
         cluster_sync();
         // the tokens of a tile are dealt to the blocks of the cluster, a warp each
@@ -265,7 +267,6 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
         cluster_sync();      // nobody leaves while others read its shared memory
     }
     if (failed && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 2);
-    if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns));
 }
 
 int tokens_per_tile(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }

@@ -380,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc5::fence_after();
     if (failed)      // a wait ran out: copies that may still be in flight get time to land
         for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     if (kSplits && p.split > 1) {
         cluster_sync();
         const Tile tile = tile_of<COLS>(p, t0);
@@ -410,7 +411,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // nothing may be left in shared memory, or on its way out of it, when the block leaves
     if (BULK && warp >= 4 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     if (failed && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 2);
-    if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 // Tensor map of the output [rows, columns] (float or bfloat16) for pieces of 32 rows x 32 bytes; what lies outside is not written.

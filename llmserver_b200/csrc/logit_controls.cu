@@ -426,13 +426,20 @@ __global__ void control_pick_kernel(const float* __restrict__ partial_scores, co
         const int other_index = __shfl_xor_sync(0xffffffffu, best_index, offset);
         take_better(best, best_index, other, other_index);
     }
-    if (lane != 0) return;
     const int token = best == -INFINITY ? -1 : best_index;
-    out[row] = token;
-    if (note && token >= 0) {
+    if (note) {
         const int at = c.history_rows[row], place = c.lengths[row];
-        if (at >= 0 && at < c.histories && place >= 0 && place < c.capacity) history[(size_t)at * c.capacity + place] = token;
+        // of rows with one place the last has it
+        bool last = true;
+        for (int other = row + 1 + lane; other < (int)gridDim.x; other += 32)
+            if (c.history_rows[other] == at && c.lengths[other] == place) last = false;
+        last = __all_sync(0xffffffffu, last);
+        if (lane == 0 && at >= c.histories && c.error_flag != nullptr) atomicExch(c.error_flag, kBadRow);
+        if (lane == 0 && last && token >= 0 && at >= 0 && at < c.histories && place >= 0 && place < c.capacity)
+            history[(size_t)at * c.capacity + place] = token;
     }
+    if (lane != 0) return;
+    out[row] = token;
     if (row == 0) leave_flags(out + gridDim.x, flag_a, flag_b);
 }
 

@@ -175,7 +175,7 @@ def sample(logits: torch.Tensor, temperatures: Optional[torch.Tensor] = None, se
 
     ``controls``: the tokens are drawn from ``control_logits(logits, controls)``, which is not written; a row whose controls leave
     nothing to draw from gets -1.  ``note``: each token drawn is written behind its request's history (history[history_rows[r],
-    lengths[r]], where there is room), after all rows' histories have been read."""
+    lengths[r]], where there is room), after all rows' histories have been read; of rows with one such place the last notes its token."""
     if controls is not None:
         return sample_controlled(logits, temperatures, seeds, steps, out, flags, controls, note)
     if note:

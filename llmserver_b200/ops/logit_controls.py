@@ -143,6 +143,9 @@ def control_logits(logits: torch.Tensor, controls: LogitControls, out: Optional[
         check(out, "controlled logits", torch.float32)
         if out.shape != logits.shape or out.device != logits.device:
             raise KernelError(f"the controlled logits {tuple(out.shape)} do not match {tuple(logits.shape)}")
+        apart = abs(out.data_ptr() - logits.data_ptr())
+        if 0 < apart < logits.numel() * 4:
+            raise KernelError("the controlled logits go to the logits' own place or to another, not to one that overlaps it")
     rows, vocab = logits.shape
     call("llm_control_logits", logits.data_ptr(), out.data_ptr(), rows, vocab, said, stream_handle())
     return out
@@ -163,6 +166,8 @@ def sample_controlled(logits: torch.Tensor, temperatures, seeds, steps, out: Opt
     if flags:
         for flag in flags:
             check(flag, "flag", torch.int32, 1)
+            if flag.get_device() != index:
+                raise KernelError(f"a flag lies on {flag.device}, the logits on {device}")
         if rows == 0:
             raise KernelError("no tokens and two flags")
     if out is None:

@@ -152,7 +152,8 @@ def test_rows_that_begin_anywhere():
 # and many blocks of k, more tiles than SMs
 SIZES = [(1, 128, 128), (1, 1, 1), (2, 16, 5), (15, 127, 129), (16, 129, 128), (17, 500, 257), (32, 512, 1000), (33, 1000, 384), (64, 640, 130),
          (65, 2001, 300), (128, 384, 1111), (129, 1024, 128), (300, 700, 700), (1000, 256, 513), (1, 4096, 6144), (8, 12288, 4096), (61, 4096, 19000),
-         (260, 8192, 260), (511, 1536, 2049), (66, 300, 40000), (1000, 384, 4100), (1290, 650, 5000), (4500, 130, 1300)]
+         (260, 8192, 260), (511, 1536, 2049), (66, 300, 40000), (1000, 384, 4100), (1290, 650, 5000), (4500, 130, 1300), (40000, 300, 100), (20001, 1500, 37),
+         (1000, 100, 20000), (37900, 128, 128)]
 
 
 @pytest.mark.parametrize("rows,inner,cols", SIZES)
@@ -296,3 +297,29 @@ def test_refusals_on_the_device():
     for call, message in cases:
         with pytest.raises(KernelError, match=message):
             call()
+
+
+def test_two_streams_at_once():
+    """Products of every form, replayed on two streams side by side again and again: the same bits as alone."""
+    shapes = [(1, 4096, 2048), (20, 2048, 1024), (64, 4096, 700), (100, 4096, 1024), (300, 1024, 3000), (900, 512, 6000)]
+    work = [(rand((rows, inner), torch.bfloat16, rows), matrix(cols, inner, cols)) for rows, inner, cols in shapes]
+    want = [ops.linear(x, weight, out_dtype=torch.float32) for x, weight in work]
+    graphs, kept = [], []
+    for order in (work, work[::-1]):
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                kept.append([ops.linear(x, weight, out_dtype=torch.float32) for _ in range(4) for x, weight in order])
+        graphs.append((graph, stream))
+    for _ in range(5):
+        for graph, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    for _, stream in graphs:
+        stream.synchronize()
+    finished()
+    for results, order in zip(kept, (want, want[::-1])):
+        for at, got in enumerate(results):
+            assert torch.equal(got, order[at % len(order)]), at

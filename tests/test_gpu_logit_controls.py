@@ -360,3 +360,50 @@ def test_refusals_on_the_device():
         ops.control_logits(logits, good(), out=torch.empty((2, 99), device=DEVICE))
     with pytest.raises(KernelError, match="temperatures"):
         ops.sample(logits, torch.ones(3, device=DEVICE), torch.zeros(3, dtype=torch.int64, device=DEVICE), whole(3), controls=good())
+
+
+def test_of_rows_with_one_place_the_last_notes_its_token():
+    """Forty rows, three of them and the last two with the same history and length; one that names no history is reported."""
+    from llmserver_b200.ops.library import KernelError, check_wait_errors
+    vocab, rows = 3000, 40
+    logits = logits_for(rows, vocab, 17)
+    controls = controls_of([Request([row], [row + 1], 1.2, 0.3, 0.1) for row in range(rows)], vocab, capacity=6)
+    for row in (9, 35):
+        controls.history_rows[row] = controls.history_rows[2]
+    controls.history_rows[rows - 2] = controls.history_rows[rows - 1]
+    before = controls.history.clone()
+    for _ in range(2):
+        controls.history.copy_(before)
+        tokens = ops.sample(logits, controls=controls, note=True)
+        finished()
+        want = before.clone()
+        for row in range(rows):      # in order, so that the last stays
+            want[int(controls.history_rows[row]), 2] = tokens[row]
+        assert torch.equal(controls.history, want)
+    controls.history.copy_(before)
+    controls.penalties, controls.history_rows[4] = None, 1000      # penalties or none: a bad index is reported
+    tokens = ops.sample(logits, controls=controls, note=True)
+    torch.cuda.synchronize()
+    with pytest.raises(KernelError, match="does not exist"):
+        check_wait_errors()
+    want = before.clone()
+    for row in range(rows):
+        if row != 4:
+            want[int(controls.history_rows[row]), 2] = tokens[row]
+    assert torch.equal(controls.history, want)
+    finished()
+
+
+def test_logits_that_overlap_their_result_are_refused():
+    from llmserver_b200.ops import KernelError
+    vocab = 100
+    room = torch.randn(300, device=DEVICE)
+    controls = controls_of([Request([1], [2], 1.5)] * 2, vocab)
+    with pytest.raises(KernelError, match="overlaps"):
+        ops.control_logits(room[:200].view(2, vocab), controls, out=room[50:250].view(2, vocab))
+    with pytest.raises(KernelError, match="overlaps"):
+        ops.control_logits(room[100:].view(2, vocab), controls, out=room[:200].view(2, vocab))
+    want = ops.control_logits(room[:200].view(2, vocab), controls)
+    got = ops.control_logits(room[:200].view(2, vocab), controls, out=room[:200].view(2, vocab))
+    finished()
+    assert torch.equal(got, want) and got.data_ptr() == room.data_ptr()
