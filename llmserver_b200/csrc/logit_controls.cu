@@ -22,7 +22,9 @@
 // slice of a row, gives -1 where nothing is left to draw from, and writes the token behind the request's history: all histories have
 // been read by then, whatever rows share one.
 //
-// What bounds it: the logits, read once (and written once by the form that returns them).
+// What bounds it: the logits, read once (and written once by the form that returns them), and behind that the block's phases, which all blocks go
+// through at the same time.  64 rows of 151936 from memory: returned 15.5 us without controls (5 TB/s) and 24.6 with histories of 4096 tokens, 50 biases
+// and masks; drawn greedily 15.3 and 22.5, at temperatures 25.0 and 30.6 (22 instructions a token for its random word and the bound).  1 row 4.8 and 8.7.
 #include "sampling.cuh"
 
 // (the caller fills this in field by field)

@@ -120,8 +120,8 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1) -> BlockScaled:
     current_device(x, "x")
     rows, columns = x.shape
     pitch = _pitch(columns)
-    values = torch.empty((rows, pitch), dtype=FLOAT8, device=x.device)
-    scales = torch.empty((_blocks(rows, block_rows), _blocks(columns)), dtype=torch.float32, device=x.device)
+    values = x.new_empty((rows, pitch), dtype=FLOAT8)
+    scales = x.new_empty((_blocks(rows, block_rows), _blocks(columns)), dtype=torch.float32)
     call("llm_quantize_blocks", x.data_ptr(), dtype_code(x.dtype), values.data_ptr(), scales.data_ptr(), rows, columns, pitch, int(block_rows),
          stream_handle())
     return BlockScaled(values if pitch == columns else values[:, :columns], scales, block_rows)
@@ -155,7 +155,7 @@ def block_linear(x, weight: BlockScaled, out: Optional[torch.Tensor] = None, out
     if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
         raise KernelError(f"block_linear writes float32 or bfloat16, not {out_dtype}")
     if out is None:
-        out = torch.empty((rows, cols), dtype=out_dtype, device=values.device)
+        out = held.new_empty((rows, cols), dtype=out_dtype)
     elif out.dtype != out_dtype or not out.is_contiguous() or tuple(out.shape) != (rows, cols):
         raise KernelError(f"block_linear: the output must be contiguous {out_dtype} [{rows}, {cols}], got {out.dtype} {tuple(out.shape)}")
     scratch = 0
@@ -163,7 +163,7 @@ def block_linear(x, weight: BlockScaled, out: Optional[torch.Tensor] = None, out
         kind, pitch, scales = -1, _row_stride(held), x.scales.data_ptr()
     else:
         kind, pitch, scales = dtype_code(x.dtype), _pitch(inner), 0
-        room = torch.empty(rows * (pitch + 4 * _blocks(inner)), dtype=torch.uint8, device=values.device)      # the rows in 8 bits, then their scales
+        room = held.new_empty(rows * (pitch + 4 * _blocks(inner)), dtype=torch.uint8)      # the rows in 8 bits, then their scales
         scratch = room.data_ptr()
     call("llm_block_linear", held.data_ptr(), kind, pitch, scales, values.data_ptr(), _row_stride(values), weight.scales.data_ptr(), out.data_ptr(),
          int(out_dtype is torch.float32), rows, cols, inner, scratch, wait_error_flag(values.device).data_ptr(), stream_handle())

@@ -171,13 +171,13 @@ def sample_controlled(logits: torch.Tensor, temperatures, seeds, steps, out: Opt
         if rows == 0:
             raise KernelError("no tokens and two flags")
     if out is None:
-        out = torch.empty(rows + (2 if flags else 0), dtype=torch.int32, device=device)
+        out = logits.new_empty(rows + (2 if flags else 0), dtype=torch.int32)
     else:
         check(out, "sampled tokens", torch.int32)
         if out.numel() != rows + (2 if flags else 0) or out.get_device() != index:
             raise KernelError(f"{rows} tokens{' and two flags' if flags else ''} do not fit {out.numel()} elements on {out.device}")
     most = rows * -(-vocab // _LEAST_SLICE)       # a score and a token for each slice of each row
-    scratch = torch.empty(2 * most, dtype=torch.float32, device=device)
+    scratch = logits.new_empty(2 * most)
     call("llm_control_sample", logits.data_ptr(), pointer(temperatures), pointer(seeds), pointer(steps), out.data_ptr(), rows, vocab, said,
          controls.history.data_ptr() if note else 0, scratch.data_ptr(), scratch.data_ptr() + 4 * most,
          *((flags[0].data_ptr(), flags[1].data_ptr()) if flags else (0, 0)), stream_handle())
