@@ -10,10 +10,14 @@
 // it leaves in pieces of 32 bytes a row while the next piece is written.  Tiles of 128 columns, where they are few, split k over a cluster; the
 // parts are added through distributed shared memory in the order of k.
 //
-// What bounds it, in SM cycles for a unit (128 of k) of 128 x 256: the MMAs alone 513, with copies, waits and signals 540, with the adders' reads
-// and 32768 products and sums 670 in a loop of nothing else; this kernel 800, of 128 x 128 620.  Counted in time the power limit comes first:
-// with random operands the SMs run at 1.3 to 1.4 GHz, and even the MMAs with their copies alone take 422 ns of the 580 of a unit.
-// 8192 x 4096 -> 24576: 752 us behind 8-bit rows, 2190 TFLOP/s; 500 x 4096 -> 4096: 14.2 us; 100 x 4096 -> 24576: 22.2 us, 4.5 TB/s.
+// A unit of the ring is a block of 128 along k for tiles of 256 columns and two blocks for tiles of 128, 48 and 64 KiB: every unit costs each role its
+// waits and signals, some 300 cycles, and both fill 256 columns of tensor memory.  (With units of a single block tiles of 128 columns took 620 cycles a
+// block, 500 x 4096 -> 4096 18.4 us and not 17.3.)
+//
+// What bounds it, in SM cycles for a unit of 128 x 256: the MMAs alone 513, with copies, waits and signals 540, with the adders' reads and 32768
+// products and sums 670 in a loop of nothing else; this kernel 800.  Counted in time the power limit comes first: with random operands the SMs run
+// at 1.3 to 1.4 GHz, and even the MMAs with their copies alone take 422 ns of the 580 of a unit.
+// 8192 x 4096 -> 24576: 745 us behind 8-bit rows, 2210 TFLOP/s; 500 x 4096 -> 4096: 13.1 us; 100 x 4096 -> 24576: 22.0 us, 4.5 TB/s.
 // Sixteen adders of half the columns take 830 to 1050 cycles, reads of 16 columns at a time 980, and sums kept as single numbers 1440 (they spill).
 //
 // Roles, bounded waits and the treatment of ragged sizes are those of gemm_block_scaled.cu.
@@ -26,9 +30,9 @@ using namespace block_scaled;
 constexpr int kTokens = 128;          // per tile (UMMA M)
 constexpr int kAdders = 8;            // warps; an adder has 32 tokens and half the columns
 constexpr int kThreads = 128 + 32 * kAdders;
-constexpr int kPart = 32;             // columns read from tensor memory at a time
-constexpr int kMaxStages = 6;
-constexpr int kMaxBuffers = 3;
+constexpr int kBuffers = 2;           // of 256 columns of tensor memory, a unit's sums
+constexpr int kRun = 4;               // most units whose scales are handed over together: a wait costs 100 cycles
+constexpr int kMaxStages = 4;
 constexpr int kMaxSplit = 4;
 constexpr int kScaleSlots = 2;        // runs of units whose scales wait to be used; another is on its way from memory
 constexpr uint32_t kXBytes = kTokens * kBlock;
@@ -39,17 +43,18 @@ struct ManyParams {
     const float* x_scales;            // [m][groups]
     const float* w_scales;            // [ceil(n / 128)][groups]
     void* out;
-    int m, n, groups;
+    int m, n, groups, units;          // blocks of 128 along k, and units of them
     int row_tiles, col_tiles, row_group;      // row tiles that are walked together for each column tile
     int split;
     int early;                        // W may be asked for before the kernel in front is complete
     int* error_flag;
 };
 
-constexpr uint32_t stage_bytes(int cols) { return kXBytes + (uint32_t)cols * kBlock; }
-constexpr int run_of(int cols) { return cols == 128 ? 8 : 4; }      // most units whose scales are handed over together: a wait costs 100 cycles
-constexpr int buffers_of(int cols) { return cols == 128 ? 3 : 2; }
-constexpr int stages_of(int cols) { return 2 * buffers_of(cols); }
+// A unit is 128 of k for tiles of 256 columns and 256 of k, two blocks, for tiles of 128.
+constexpr int blocks_of(int cols) { return 256 / cols; }
+constexpr uint32_t stage_bytes(int cols) { return (uint32_t)blocks_of(cols) * (kXBytes + (uint32_t)cols * kBlock); }
+constexpr int stages_of(int cols) { return cols == 128 ? 3 : 4; }
+constexpr int lap_of(int cols) { return cols == 128 ? 6 : 4; }      // units after which stages and buffers are where they were
 constexpr uint32_t shared_bytes(int cols) { return stages_of(cols) * stage_bytes(cols) + kAdders * 2 * kPieceBytes + 1024; }
 
 // Tile t of the walk: row_group row tiles through all column tiles before the next ones, so that these rows of x stay in L2 while W passes.
@@ -66,16 +71,16 @@ __device__ __forceinline__ Tile tile_of(const ManyParams& p, int t) {
 // The units of this block, one after the other.
 template <int COLS>
 struct Walk {
-    int t, group, first, last;
+    int t, unit, first, last;
     Tile tile;
     __device__ __forceinline__ void begin(const ManyParams& p, int t0, int from, int to) {
-        t = t0, group = first = from, last = to;
+        t = t0, unit = first = from, last = to;
         tile = tile_of<COLS>(p, t);
     }
-    __device__ __forceinline__ bool ends() const { return group + 1 == last; }
+    __device__ __forceinline__ bool ends() const { return unit + 1 == last; }
     __device__ __forceinline__ void step(const ManyParams& p, int stride, int total) {
-        if (++group < last) return;
-        group = first;
+        if (++unit < last) return;
+        unit = first;
         t += stride;
         if (t < total) tile = tile_of<COLS>(p, t);
     }
@@ -151,22 +156,21 @@ template <int COLS, int ELEMENT, bool BULK>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_block_scaled_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                   const __grid_constant__ CUtensorMap map_out, const ManyParams p) {
-    constexpr int kBuffers = buffers_of(COLS), kStages = stages_of(COLS), kHalves = COLS / 128, kWidth = COLS / 2;
-    constexpr int kRun = run_of(COLS);
-    constexpr uint32_t kStageBytes = stage_bytes(COLS);
+    constexpr int kStages = stages_of(COLS), kLap = lap_of(COLS), kBlocks = blocks_of(COLS), kWidth = COLS / 2;
+    constexpr uint32_t kStageBytes = stage_bytes(COLS), kWBytes = COLS * kBlock, kUnitW = kBlocks * kXBytes;      // the last: where a stage's W begins
     constexpr bool kSplits = COLS == 128;      // the narrow tiles alone
-    static_assert(kBuffers <= kMaxBuffers && kStages <= kMaxStages, "the barriers are enough");
+    static_assert(kStages <= kMaxStages && kLap % kStages == 0 && kLap % kBuffers == 0, "the barriers are enough, and a lap is whole");
     extern __shared__ unsigned char many_shared[];
-    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], sums_bars[2][kMaxBuffers],
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], sums_bars[2][kBuffers],
         scale_full[kScaleSlots], scale_empty[kScaleSlots];
-    __shared__ float scales[kScaleSlots][kRun][kHalves][kTokens];      // of a unit: each token's times W's
+    __shared__ float scales[kScaleSlots][kRun][2][kTokens];      // of a unit's two blocks of W: each token's times W's
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
     const uint32_t ring = (tma::smem_u32(many_shared) + 1023u) & ~1023u;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = kSplits && p.split > 1 ? (int)cluster_rank() : 0, in_cluster = kSplits ? p.split : 1;
     const int total = p.row_tiles * p.col_tiles, stride = (int)gridDim.x / in_cluster, t0 = (int)blockIdx.x / in_cluster;
-    const int first = (int)((long long)p.groups * rank / in_cluster), last = (int)((long long)p.groups * (rank + 1) / in_cluster);
+    const int first = (int)((long long)p.units * rank / in_cluster), last = (int)((long long)p.units * (rank + 1) / in_cluster);
     const int tiles = (total - t0 + stride - 1) / stride, count = tiles * (last - first);      // this block's units
     Walk<COLS> walk;
     walk.begin(p, t0, first, last);
@@ -192,7 +196,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         Walk<COLS> ahead = walk;
         for (int s = 0; s < kStages && s < count; ++s) {
             tma::mbar_expect_tx(tma::smem_u32(&full[s]), kStageBytes);
-            tma::load_2d(ring + s * kStageBytes + kXBytes, &map_w, tma::smem_u32(&full[s]), ahead.group * kBlock, ahead.tile.col0);
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k)
+                tma::load_2d(ring + s * kStageBytes + kUnitW + k * kWBytes, &map_w, tma::smem_u32(&full[s]), (ahead.unit * kBlocks + k) * kBlock, ahead.tile.col0);
             ahead.step(p, stride, total);
         }
     }
@@ -211,18 +217,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
         if (elect_one()) {
             bool ok = true;
-            uint32_t lap = 0;      // of the ring; a stage's barriers complete once a lap
-            for (int i0 = 0; i0 < count && ok; i0 += kStages, ++lap) {
+            uint32_t lap = 0;      // of stages and buffers; a stage's barriers complete kLap / kStages times in it
+            for (int i0 = 0; i0 < count && ok; i0 += kLap, ++lap) {
 #pragma unroll
-                for (int s = 0; s < kStages; ++s) {
-                    const uint32_t stage = ring + s * kStageBytes, bar = tma::smem_u32(&full[s]);
+                for (int s = 0; s < kLap; ++s) {
+                    const int at = s % kStages;
+                    const uint32_t stage = ring + at * kStageBytes, bar = tma::smem_u32(&full[at]), turn = lap * (kLap / kStages) + s / kStages;
                     if (i0 + s >= count) break;
-                    if (lap > 0 && !(ok = tma::mbar_wait(tma::smem_u32(&empty[s]), (lap & 1) ^ 1))) break;
-                    if (!p.early || lap > 0) {
-                        tma::mbar_expect_tx(bar, kStageBytes);
-                        tma::load_2d(stage + kXBytes, &map_w, bar, walk.group * kBlock, walk.tile.col0);
+                    if (turn > 0 && !(ok = tma::mbar_wait(tma::smem_u32(&empty[at]), (turn & 1) ^ 1))) break;
+                    if (!p.early || turn > 0) tma::mbar_expect_tx(bar, kStageBytes);
+#pragma unroll
+                    for (int k = 0; k < kBlocks; ++k) {      // what lies beyond the last of k is zeros
+                        const int x = (walk.unit * kBlocks + k) * kBlock;
+                        if (!p.early || turn > 0) tma::load_2d(stage + kUnitW + k * kWBytes, &map_w, bar, x, walk.tile.col0);
+                        tma::load_2d(stage + k * kXBytes, &map_x, bar, x, walk.tile.token0);
                     }
-                    tma::load_2d(stage, &map_x, bar, walk.group * kBlock, walk.tile.token0);
                     walk.step(p, stride, total);
                 }
             }
@@ -232,28 +241,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) failed = 1;
         }
     } else if (warp == 1) {
-        // A lap of the ring is written out, so that every place, buffer and parity but the ring's own is a constant, and one lane walks it: with
-        // places counted up beside the warp's vote a unit took this warp 390 cycles with one wait and no work for anybody else, like this 297.
+        // A lap is written out, so that every place and buffer is a constant, and one lane walks it: with places counted up beside the warp's vote a
+        // unit took this warp 390 cycles with one wait and no work for anybody else, like this 297.
         if (elect_one()) {
             const uint32_t idesc = instruction_f8(kTokens, COLS);
-            const uint64_t desc_x = tc5::desc_k_major(ring, 1024u), desc_w = tc5::desc_k_major(ring + kXBytes, 1024u);
+            const uint64_t desc_x = tc5::desc_k_major(ring, 1024u), desc_w = tc5::desc_k_major(ring + kUnitW, 1024u);
             bool ok = true;
             uint32_t lap = 0;
-            for (int i0 = 0; i0 < count && ok; i0 += kStages, ++lap) {
+            for (int i0 = 0; i0 < count && ok; i0 += kLap, ++lap) {
 #pragma unroll
-                for (int s = 0; s < kStages; ++s) {
-                    constexpr uint64_t kStep = kStageBytes >> 4;      // descriptors hold addresses in units of 16 bytes
+                for (int s = 0; s < kLap; ++s) {
+                    const int at = s % kStages, b = s % kBuffers;
+                    const uint32_t turn = lap * (kLap / kBuffers) + s / kBuffers;      // of the buffer
                     if (i0 + s >= count) break;
-                    const int b = s % kBuffers;      // used twice a lap
-                    ok = tma::mbar_wait(tma::smem_u32(&full[s]), lap & 1);
-                    if (ok && (s >= kBuffers || lap > 0)) ok = tma::mbar_wait(tma::smem_u32(&sums_bars[1][b]), s < kBuffers);
+                    ok = tma::mbar_wait(tma::smem_u32(&full[at]), (lap * (kLap / kStages) + s / kStages) & 1);
+                    if (ok && (s >= kBuffers || lap > 0)) ok = tma::mbar_wait(tma::smem_u32(&sums_bars[1][b]), (turn & 1) ^ 1);
                     if (!ok) break;
                     tc5::fence_after();
 #pragma unroll
-                    for (int k = 0; k < kBlock / 32; ++k)
-                        mma_f8(tmem + b * COLS, desc_x + s * kStep + k * 2, desc_w + s * kStep + k * 2, idesc, k > 0);
+                    for (int k = 0; k < kBlocks * (kBlock / 32); ++k) {
+                        const int block = k / (kBlock / 32), in_block = k % (kBlock / 32);
+                        // descriptors hold addresses in units of 16 bytes
+                        const uint64_t x_at = (at * kStageBytes + block * kXBytes) >> 4, w_at = (at * kStageBytes + block * kWBytes) >> 4;
+                        mma_f8(tmem + b * 256 + block * COLS, desc_x + x_at + in_block * 2, desc_w + w_at + in_block * 2, idesc, in_block > 0);
+                    }
                     tc5::mma_commit(tma::smem_u32(&sums_bars[0][b]));
-                    tc5::mma_commit(tma::smem_u32(&empty[s]));
+                    tc5::mma_commit(tma::smem_u32(&empty[at]));
                 }
             }
             if (!ok) failed = 1;
@@ -262,16 +275,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         // A lane's four tokens' scales times W's, asked for a run of units before: up to kRun units of one tile.  (Addresses are made once a tile: with
         // them and their bounds made for each unit a unit took 20 cycles more.)
         const int col_blocks = (p.n + 127) / 128;
-        const float *x_from[4], *w_from[kHalves];
-        float x_scale[kRun][4], w_scale[kRun][kHalves];
-        int t = t0, next = last;      // the tile and the group to ask for next
+        const float *x_from[4], *w_from[2 / kBlocks];
+        float x_scale[kRun][kBlocks][4], w_scale[kRun][2];
+        int t = t0, next = last;      // the tile and the unit to ask for next
         auto ask = [&](int units) {
             if (next == last) {      // a new tile; what lies outside the matrices reads something that does not
                 const Tile tile = tile_of<COLS>(p, t);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x_from[j] = p.x_scales + (size_t)min(tile.token0 + j * 32 + lane, p.m - 1) * p.groups;
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h) w_from[h] = p.w_scales + (size_t)min(tile.col0 / 128 + h, col_blocks - 1) * p.groups;
+                for (int h = 0; h < 2 / kBlocks; ++h) w_from[h] = p.w_scales + (size_t)min(tile.col0 / 128 + h, col_blocks - 1) * p.groups;
                 t += stride;
                 next = first;
             }
@@ -279,9 +292,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int d = 0; d < kRun; ++d)
                 if (d < units) {
 #pragma unroll
-                    for (int h = 0; h < kHalves; ++h) w_scale[d][h] = w_from[h][next + d];
+                    for (int k = 0; k < kBlocks; ++k) {      // beyond the last block of k there are zeros to be multiplied
+                        const int group = (next + d) * kBlocks + k;
+                        const bool there = kBlocks == 1 || group < p.groups;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x_scale[d][j] = x_from[j][next + d];
+                        for (int h = 0; h < 2 / kBlocks; ++h) w_scale[d][kBlocks == 1 ? h : k] = there ? w_from[h][group] : 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x_scale[d][k][j] = there ? x_from[j][group] : 0.0f;
+                    }
                 }
             next += units;
         };
@@ -295,9 +313,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int d = 0; d < kRun; ++d)
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) scales[slot.at][d][h][j * 32 + lane] = x_scale[d][j] * w_scale[d][h];
+                    for (int j = 0; j < 4; ++j) scales[slot.at][d][h][j * 32 + lane] = x_scale[d][kBlocks == 1 ? 0 : h][j] * w_scale[d][h];
             i += units;
             units = next == last ? min(kRun, last - first) : min(kRun, last - next);
             if (i < count) ask(units);
@@ -313,40 +331,48 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < kWidth / 2; ++c) sums[c] = 0;
         // Addresses and parities go on by additions, in registers of the lanes, which the shuffle keeps them in: with places counted up and multiplied
-        // with sizes, in the warp's uniform registers, a unit of 128 columns took 795 cycles and not 670, of 256 columns 885 and not 825.
+        // with sizes, in the warp's uniform registers, a unit of 256 columns took 885 cycles and not 825.
         const uint32_t vary = (uint32_t)__shfl_sync(0xffffffffu, 0, lane);      // 0
-        const uint32_t bars = tma::smem_u32(&sums_bars[0][0]) + vary, my_scales = tma::smem_u32(&scales[0][0][kHalves == 2 ? share : 0][quarter * 32 + lane]);
+        const uint32_t bars = tma::smem_u32(&sums_bars[0][0]) + vary, my_scales = tma::smem_u32(&scales[0][0][kBlocks == 1 ? share : 0][quarter * 32 + lane]);
         uint32_t bar = bars, parity = vary, from = address;      // of the buffer: sums_full's address
         bool ok = true;
         Turn slot;
         for (int t = t0; t < total && ok; t += stride) {
-            for (int group = first; group < last && ok; group += kRun) {
+            for (int unit = first; unit < last && ok; unit += kRun) {
                 uint32_t scale_at = my_scales + slot.at * (uint32_t)sizeof(scales[0]);
                 ok = tma::mbar_wait(tma::smem_u32(&scale_full[slot.at]), slot.parity);
 #pragma unroll 1
-                for (int units = min(kRun, last - group); units > 0; --units) {
-                    float scale;
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(scale_at) : "memory");
+                for (int units = min(kRun, last - unit); units > 0; --units) {
+                    float scale[kBlocks];
+#pragma unroll
+                    for (int k = 0; k < kBlocks; ++k) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale[k]) : "r"(scale_at + k * kTokens * 4) : "memory");
                     scale_at += (uint32_t)sizeof(scales[0][0]);
                     ok = __all_sync(0xffffffffu, ok && tma::mbar_wait(bar, parity));
                     if (!ok) break;
                     tc5::fence_after();
-                    const uint64_t both = tc5::pair_of(scale, scale);
+                    // read from tensor memory at a time: 32 columns, or with half the sums to hold a block's 64
+                    constexpr int kPart = kBlocks == 1 ? 32 : 64;
 #pragma unroll
-                    for (int part = 0; part < kWidth; part += kPart) {
-                        uint32_t r[kPart];
-                        tmem_ask<kPart>(from + part, r);
-                        tmem_wait<kPart>(r);
-                        if (part + kPart == kWidth) {      // all of the buffer is in registers
+                    for (int part = 0; part < 128; part += kPart) {
+                        const int k = kBlocks == 1 ? 0 : part / kWidth, first_column = kBlocks == 1 ? part : 0;
+                        uint32_t r[kPart / 32][32];
+#pragma unroll
+                        for (int c = 0; c < kPart; c += 32) tmem_ask<32>(from + k * COLS + first_column + c, r[c / 32]);
+#pragma unroll
+                        for (int c = 0; c < kPart; c += 32) tmem_wait<32>(r[c / 32]);
+                        if (part + kPart == 128) {      // all of the buffer is in registers
                             tc5::fence_before();
                             __syncwarp();
-                            if (lane == 0) tma::mbar_arrive(bar + kMaxBuffers * 8);
+                            if (lane == 0) tma::mbar_arrive(bar + kBuffers * 8);
                         }
+                        const uint64_t both = tc5::pair_of(scale[k], scale[k]);
 #pragma unroll
-                        for (int c = 0; c < kPart; c += 2)
-                            sums[(part + c) / 2] = tc5::fma_pair(tc5::pair_of(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), both, sums[(part + c) / 2]);
+                        for (int c = 0; c < kPart; c += 2) {
+                            uint64_t& sum = sums[(first_column + c) / 2];
+                            sum = tc5::fma_pair(tc5::pair_of(__uint_as_float(r[c / 32][c % 32]), __uint_as_float(r[c / 32][c % 32 + 1])), both, sum);
+                        }
                     }
-                    bar += 8, from += COLS;
+                    bar += 8, from += 256;
                     if (bar == bars + kBuffers * 8) bar = bars, from = address, parity ^= 1;
                 }
                 __syncwarp();
@@ -436,13 +462,14 @@ int launch_many(const CUtensorMap& map_x, const CUtensorMap& map_out, const void
     const int places = llm_sm_count();
     p.row_tiles = (p.m + kTokens - 1) / kTokens;
     p.col_tiles = (p.n + COLS - 1) / COLS;
+    p.units = (p.groups + blocks_of(COLS) - 1) / blocks_of(COLS);
     const long long total = (long long)p.row_tiles * p.col_tiles;
     // row tiles whose rows of x stay in L2 together while W passes: at most 32 MiB of them
     const long long fit = (32LL << 20) / ((long long)kTokens * inner);
     p.row_group = (int)(fit < 1 ? 1 : fit < p.row_tiles ? fit : p.row_tiles);
     p.split = 1;
     if (COLS == 128)
-        while (2 * p.split <= kMaxSplit && total * 2 * p.split <= places && p.groups / (2 * p.split) >= 4) p.split *= 2;
+        while (2 * p.split <= kMaxSplit && total * 2 * p.split <= places && p.units / (2 * p.split) >= 2) p.split *= 2;
     const size_t shared = shared_bytes(COLS);
     if (int status = llm_raise_shared_limit((const void*)gemm_block_scaled_many_kernel<COLS, ELEMENT, BULK>, shared, "block_linear", true)) return status;
     cudaLaunchConfig_t config = {};
@@ -489,11 +516,11 @@ int llm_block_linear_many(const void* x, long long x_pitch, const float* x_scale
         return LLM_REFUSED;
     }
     if (!bulk) map_out = map_x;      // not used
-    // A unit of a tile of 256 columns takes 800 cycles, of 128 columns 620: the wider ones unless the narrower ones fill the SMs better by more than
-    // that (384 x 4096 -> 6144, one tile an SM either way: 18.9 us narrow, 22.3 wide; 700 rows, 2 and 1: 29.7 and 23.3).
+    // A block of k of a tile of 256 columns takes 800 cycles, of 128 columns 530: the wider ones unless the narrower ones fill the SMs better by that
+    // (384 x 4096 -> 6144, one tile an SM either way: 17.1 us narrow, 22.3 wide; 900 rows, 3 and 2: 35.8 and 37.9; 700 rows, 2 and 1: 28.9 and 23.5).
     const long long sms = llm_sm_count(), rows = (m + kTokens - 1) / kTokens;
     const long long wide = (rows * ((n + 255) / 256) + sms - 1) / sms, narrow = (rows * ((n + 127) / 128) + sms - 1) / sms;
-    const int form = 4 * narrow < 5 * wide ? 0 : 1;
+    const int form = 2 * narrow <= 3 * wide ? 0 : 1;
     using Launch = int (*)(const CUtensorMap&, const CUtensorMap&, const void*, long long, ManyParams, int, cudaStream_t);
     static const Launch launches[2][2][2] = {
         {{launch_many<128, 2, false>, launch_many<128, 2, true>}, {launch_many<128, 4, false>, launch_many<128, 4, true>}},
