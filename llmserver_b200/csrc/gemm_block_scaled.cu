@@ -5,7 +5,7 @@
 // multiplied with the block's two scales and added up in registers, 32-bit as well: the scales are any 32-bit numbers, so blocks
 // cannot be added before they are scaled.
 //
-// For up to 64 tokens (more: gemm_block_scaled_many.cu).  The roles of the operands are swapped for the hardware, as in gemm_tcgen05.cu:
+// For up to 64 tokens (more, and from 33 on large matrices: gemm_block_scaled_many.cu).  The roles of the operands are swapped for the hardware, as in gemm_tcgen05.cu:
 // 128 rows of W are the MMA's M, the tokens (16, 32 or 64) its N, so that a product of few tokens streams W and wastes nothing on rows
 // that do not exist.  A stage of the ring is one block of 128 along k: 16 KiB of W and 2 to 8 KiB of x, which are one swizzle atom wide.  The MMAs of a block go to one of several
 // buffers of tensor memory, so that they run ahead of the warps that scale and add.
@@ -29,7 +29,6 @@ namespace {
 using namespace block_scaled;
 
 constexpr int kRows = 128;            // rows of W per tile (UMMA M)
-constexpr int kMany = 64;             // beyond so many tokens they are the MMA's M (gemm_block_scaled_many.cu)
 constexpr int kAdders = 4;            // warps that scale and add
 constexpr int kThreads = 128 + 32 * kAdders;
 constexpr int kPerSm = 2;             // blocks that share an SM: one streams while the other begins or ends
@@ -272,6 +271,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     if (failed && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 2);
 }
 
+// Whether the tokens are the MMA's M (gemm_block_scaled_many.cu): beyond 64 of them, and beyond 32 where W's tiles are enough for every other SM, so that
+// that kernel need not split k (40 rows by 8192 x 2048 11.4 us here and 12.6 there, by 10240 x 4096 15.8 and 15.0, by 24576 x 4096 25.3 and 23.4; 64 rows
+// by 4096 x 4096 13.4 and 13.7, by 24576 x 4096 26.9 and 23.7; 32 rows by 24576 x 4096, in tiles of 32, 22.4 here).
+bool many_rows(int m, int n) { return m > 64 || (m > 32 && 2 * ((n + kRows - 1LL) / kRows) > llm_sm_count()); }
+
 int tokens_per_tile(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
 
 // Into how many parts k is split: as many as one round of blocks holds (a second round waits for the first to give up its share of an SM:
@@ -372,7 +376,7 @@ LLM_EXPORT int llm_block_linear(const void* x, int x_dtype, long long x_pitch, c
         p.x_scales = made;
         p.early = 1;      // that kernel lets this one in only when all in front of it is complete
     }
-    if (m > kMany)
+    if (many_rows(m, n))
         return llm_block_linear_many(rows, x_pitch, p.x_scales, w, w_pitch, w_scales, out, out_is_f32, m, n, inner, p.early, error_flag, stream);
     switch (tokens_per_tile(m)) {
         case 16: return launch_block_scaled<16>(rows, x_pitch, w, w_pitch, p, inner, stream);

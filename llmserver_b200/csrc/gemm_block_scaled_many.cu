@@ -77,7 +77,6 @@ struct Walk {
         t = t0, unit = first = from, last = to;
         tile = tile_of<COLS>(p, t);
     }
-    __device__ __forceinline__ bool ends() const { return unit + 1 == last; }
     __device__ __forceinline__ void step(const ManyParams& p, int stride, int total) {
         if (++unit < last) return;
         unit = first;
