@@ -24,7 +24,7 @@
 //
 // What bounds it: the logits, read once (and written once by the form that returns them), and behind that the block's phases, which all blocks go
 // through at the same time.  64 rows of 151936 from memory: returned 15.5 us without controls (5 TB/s) and 24.6 with histories of 4096 tokens, 50 biases
-// and masks; drawn greedily 15.3 and 22.5, at temperatures 25.0 and 30.6 (22 instructions a token for its random word and the bound).  1 row 4.8 and 8.7.
+// and masks; drawn greedily 15.3 and 22.5, at temperatures 24.3 and 30.0 (20 instructions a token for its random word and the bound).  1 row 4.8 and 8.7.
 #include "sampling.cuh"
 
 // (the caller fills this in field by field)
@@ -215,24 +215,27 @@ __device__ __forceinline__ int ordered(float v) {
 }
 __device__ __forceinline__ float unordered(int v) { return __int_as_float(v >= 0 ? v : v ^ 0x7fffffff); }
 
-// The draw of a row at a temperature.  Most tokens cannot win, and an upper bound of their score says so for a fifth of its price:
-// with u = 1 - v, -log u >= v, so that the noise -log(-log u) is at most -log v.  The bound's own errors (the approximate logarithm's, the
-// product's for the quotient) are below a thousandth and a millionth of the score, which it is raised by.
+// The draw of a row at a temperature.  Most tokens cannot win, and an upper bound of their score says so for a fifth of its price: with
+// u = 1 - v, -log u >= v, so that the noise -log(-log u) is at most -log v, which is below 17.  The bound's own errors (the approximate logarithm's,
+// the product's for the quotient) are below a thousandth and a millionth of the quotient, and a quotient that needs noise to reach a score is within 17 of
+// it: the score is lowered by as much, once for many tokens.
 struct Draw {
     float temperature, inverse;
     uint32_t word;      // of seed and step
     __device__ __forceinline__ void begin(float t, uint64_t seed, uint32_t step) {
         temperature = t;
         inverse = 1.0f / t;
+        if (inverse > 3.4028234e38f) inverse = NAN;      // a temperature below the normal numbers: no bound
         word = mix32(mix32(mix32((uint32_t)seed ^ 0x9E3779B9u) ^ (uint32_t)(seed >> 32)) ^ step);
     }
-    __device__ __forceinline__ bool may_exceed(float logit, int token, float best) const {
+    // What the bound of a token that may reach `best` is not below.
+    static __device__ __forceinline__ float floor_of(float best) { return best - fmaf(fabsf(best) + 17.0f, 1e-6f, 1e-3f); }
+    __device__ __forceinline__ bool may_reach(float logit, int token, float floor) const {
         const uint32_t k = mix32(word ^ (uint32_t)token) >> 9;
-        const float v = (2.0f - __uint_as_float(0x3f800000u | k)) - 1.0f / 16777216.0f;      // exact: 1 - (k + 1/2) / 2^23
+        const float v = 1.99999988f - __uint_as_float(0x3f800000u | k);      // exact: 1 - (k + 1) / 2^23, a little below 1 - u
         float log2_v;
         asm("lg2.approx.f32 %0, %1;" : "=f"(log2_v) : "f"(v));
-        const float scaled = logit * inverse;
-        return !(fmaf(-0.69314718f, log2_v, scaled) + fmaf(fabsf(scaled), 1e-6f, 1e-3f) < best);      // true where anything is a NaN
+        return !(fmaf(-0.69314718f, log2_v, logit * inverse) < floor);      // true where anything is a NaN
     }
     __device__ __forceinline__ float score(float logit, int token) const {
         const uint32_t k = mix32(word ^ (uint32_t)token) >> 9;
@@ -348,10 +351,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* 
                 __syncthreads();
                 from = 1;
             }
-            const float set = unordered(bar);
+            const float set = unordered(bar), floor = Draw::floor_of(fmaxf(best, set));
 #pragma unroll
             for (int a = 0; a < kAhead; ++a)
-                if (a >= from && now[a] > -INFINITY && draw.may_exceed(now[a], token(a), fmaxf(best, set))) take(a);
+                if (a >= from && now[a] > -INFINITY && draw.may_reach(now[a], token(a), floor)) take(a);
             if (best > set) atomicMax(&bar, ordered(best));      // for everybody's next laps
         } else {
             float high = now[0];

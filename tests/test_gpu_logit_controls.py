@@ -407,3 +407,20 @@ def test_logits_that_overlap_their_result_are_refused():
     got = ops.control_logits(room[:200].view(2, vocab), controls, out=room[:200].view(2, vocab))
     finished()
     assert torch.equal(got, want) and got.data_ptr() == room.data_ptr()
+
+
+@pytest.mark.parametrize("temperature", [1e-39, 1e-30, 1e-3, 0.3, 30.0, 1e30])
+@pytest.mark.parametrize("shift,scale", [(0.0, 3.0), (-1e4, 1.0), (1e6, 50.0), (-1e-3, 1e-4)])
+def test_draws_at_any_temperature_are_those_without_controls(temperature, shift, scale):
+    """Controls that change nothing: tokens are passed over by a bound of their scores here and worked out one by one there."""
+    rows, vocab = 6, 20000
+    logits = logits_for(rows, vocab, 23) * scale + shift
+    temperatures = torch.full((rows,), temperature, dtype=torch.float32, device=DEVICE)
+    seeds, steps = torch.arange(rows, device=DEVICE), torch.arange(rows, dtype=torch.int32, device=DEVICE)
+    want = ops.sample(logits, temperatures, seeds, steps)
+    everything = torch.ones(vocab, dtype=torch.bool)
+    got = ops.sample(logits, temperatures, seeds, steps, controls=controls_of([Request(allowed=everything)] * rows, vocab))
+    finished()
+    scores = logits.double() / float(temperatures[0])
+    drawn = (scores.abs().max(1).values < torch.finfo(torch.float32).max).tolist()      # where no score is infinite
+    assert [int(g) for g, d in zip(got, drawn) if d] == [int(w) for w, d in zip(want, drawn) if d]
