@@ -323,3 +323,31 @@ def test_two_streams_at_once():
     for results, order in zip(kept, (want, want[::-1])):
         for at, got in enumerate(results):
             assert torch.equal(got, order[at % len(order)]), at
+
+
+def quantized_rows(x):
+    """``quantized(x, 1)`` for many rows: all blocks at a time, finite numbers only."""
+    rows, columns = x.shape
+    groups = -(-columns // 128)
+    blocks = torch.nn.functional.pad(x.double(), (0, groups * 128 - columns)).view(rows, groups, 128)
+    mantissa, exponent = torch.frexp(blocks.abs().amax(2))      # 448 is 0.875 times 2^9
+    exponent = torch.where(mantissa > 0.875, exponent - 8, torch.where(mantissa > 0, exponent - 9, -126)).clamp(min=-126)
+    scales = torch.ldexp(torch.ones_like(mantissa), exponent)
+    return nearest(blocks / scales[:, :, None]).reshape(rows, groups * 128)[:, :columns], scales
+
+
+@pytest.mark.parametrize("rows,columns", [(7, 130), (2400, 4104), (19001, 504), (80000, 8), (77000, 100), (1300, 8200), (600, 12345)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows_that_end_inside_a_block(rows, columns, dtype):
+    """More groups than half warps run at a time, several times over."""
+    x = rand((rows, columns), dtype, 31)
+    x[rows // 2] = 0
+    x[rows - 1, columns - 1] = 1e4
+    got = ops.quantize_blocks(x)
+    finished()
+    want_values, want_scales = quantized_rows(x)
+    if rows < 10:
+        same(want_values, quantized(x, 1)[0].float())
+        same(want_scales, quantized(x, 1)[1].float())
+    same(got.values, want_values)
+    same(got.scales, want_scales)
