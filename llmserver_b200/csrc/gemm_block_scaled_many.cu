@@ -12,7 +12,7 @@
 //
 // A unit of the ring is a block of 128 along k for tiles of 256 columns and two blocks for tiles of 128, 48 and 64 KiB: every unit costs each role its
 // waits and signals, some 300 cycles, and both fill 256 columns of tensor memory.  (With units of a single block tiles of 128 columns took 620 cycles a
-// block, 500 x 4096 -> 4096 18.4 us and not 17.3.)
+// block, 500 x 4096 -> 4096 14.2 us behind 8-bit rows and not 13.1.)
 //
 // What bounds it, in SM cycles for a unit of 128 x 256: the MMAs alone 513, with copies, waits and signals 540, with the adders' reads and 32768
 // products and sums 670 in a loop of nothing else; this kernel 800.  Counted in time the power limit comes first: with random operands the SMs run
