@@ -137,6 +137,13 @@ class StepFunction:
         clock = time.perf_counter
         began = clock()
         slices = self.slices_for(entries)
+        allowed = None
+        if steered is not None:
+            # a grammar is the caller's and may raise: it is asked before the model runs, which replaces recurrent states in place, so
+            # that the step can be run again
+            if self.controls is None:
+                self.controls = ControlTable(self.device, self.model.spec.vocab_size)
+            allowed = self.controls.allowed(steered)
         graph = self.graphs.ready_for(slices) if self.graphs is not None and sampling else None
         advanced = False
 
@@ -148,12 +155,10 @@ class StepFunction:
 
         described = None
 
-        def describe() -> None:     # before anything moves on: a grammar of the caller's may raise
+        def describe() -> None:     # while the GPU works: nothing of the caller's is called here
             nonlocal described
             if steered is not None:
-                if self.controls is None:
-                    self.controls = ControlTable(self.device, self.model.spec.vocab_size)
-                described = self.controls.describe(steered)
+                described = self.controls.describe(steered, allowed)
 
         def meanwhile() -> None:
             describe()

@@ -100,9 +100,27 @@ class ControlTable:
             self.noted.clear()
         return place
 
-    def describe(self, requests: Sequence) -> ops.LogitControls:
+    def allowed(self, requests: Sequence) -> List[Optional[np.ndarray]]:
+        """Asks the grammars of a step's rows: per row the words of its mask, or None where all tokens are allowed.  What a grammar raises goes on
+        to the caller with a note that names the request; nothing has changed here by then."""
+        found: List[Optional[np.ndarray]] = []
+        for request in requests:
+            words = None
+            if request is not None and request.controls.allowed_tokens is not None:
+                try:
+                    given = request.controls.allowed_tokens(list(request.generated_token_ids))
+                except Exception as error:
+                    error.add_note(f"raised by allowed_tokens of request {request.request_id!r}")
+                    raise
+                words = None if given is None else mask_words(given, self.vocab)
+            found.append(words)
+        return found
+
+    def describe(self, requests: Sequence, allowed: Optional[Sequence] = None) -> ops.LogitControls:
         """The controls of a step's rows; ``requests``: per row a request with ``controls``, ``request_id``, ``prompt_token_ids`` and
-        ``generated_token_ids``, or None for a row without controls."""
+        ``generated_token_ids``, or None for a row without controls.  ``allowed``: what ``allowed`` gave for them (default: it is asked)."""
+        if allowed is None:
+            allowed = self.allowed(requests)
         count = len(requests)
         packed = np.zeros((8, count), dtype=np.int32)      # history, bias and mask rows, length, prompt length, then the penalties
         packed[:3] = -1
@@ -122,11 +140,9 @@ class ControlTable:
                 placed.append((request, held))
             if controls.logit_bias:
                 packed[1, row] = biased.index(request)
-            if controls.allowed_tokens is not None:
-                allowed = controls.allowed_tokens(list(request.generated_token_ids))
-                if allowed is not None:
-                    packed[2, row] = len(masks)
-                    masks.append(mask_words(allowed, self.vocab))
+            if allowed[row] is not None:
+                packed[2, row] = len(masks)
+                masks.append(allowed[row])
         for request, held in placed:      # (behind all rows: the table may have grown)
             if self.noted.get(request.request_id) != held:
                 tokens = np.asarray(list(request.prompt_token_ids) + list(request.generated_token_ids), dtype=np.int32)
