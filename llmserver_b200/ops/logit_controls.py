@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import struct
 from dataclasses import dataclass
-from typing import Mapping, Optional, Sequence
+from typing import Dict, Mapping, Optional, Sequence
 
 import torch
 
@@ -184,15 +184,35 @@ def sample_controlled(logits: torch.Tensor, temperatures, seeds, steps, out: Opt
     return out
 
 
+def biases_by_token(entries: Mapping, vocab: int) -> Dict[int, float]:
+    """Token -> bias in ascending order.  The keys are whole numbers, or texts of such, which JSON makes of them; raises ValueError for any
+    other, for tokens outside the vocabulary and for a token that is named twice."""
+    found = {}
+    for key, value in entries.items():
+        try:
+            token = int(key)
+        except (TypeError, ValueError, OverflowError):
+            token = None
+        if token is None or (not isinstance(key, str) and token != key):
+            raise ValueError(f"a bias for {key!r}, which is no token")
+        if not 0 <= token < vocab:
+            raise ValueError(f"a bias for token {token}, which is outside the vocabulary of {vocab}: tokens are 0 to {vocab - 1}")
+        if token in found:
+            raise ValueError(f"two biases for token {token}")
+        found[token] = float(value)
+    return dict(sorted(found.items()))
+
+
 def bias_lists(biases: Sequence[Mapping[int, float]], vocab: int, device) -> dict:
     """``bias_starts``, ``bias_ids`` and ``bias_values`` of ``LogitControls`` for one mapping (token -> bias) per list."""
     starts, ids, values = [0], [], []
     for index, entries in enumerate(biases):
-        for token in sorted(entries):
-            if not 0 <= int(token) < vocab:
-                raise KernelError(f"bias list {index}: token {token} is outside the vocabulary of {vocab}")
-            ids.append(int(token))
-            values.append(float(entries[token]))
+        try:
+            whole = biases_by_token(entries, vocab)
+        except ValueError as error:
+            raise KernelError(f"bias list {index}: {error}") from error
+        ids.extend(whole)
+        values.extend(whole.values())
         starts.append(len(ids))
     return {"bias_starts": torch.tensor(starts, dtype=torch.int32, device=device), "bias_ids": torch.tensor(ids, dtype=torch.int32, device=device),
             "bias_values": torch.tensor(values, dtype=torch.float32, device=device)}

@@ -7,21 +7,23 @@ controls, draws a token and notes it.  The reference samples greedily without an
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import Callable, Dict, List, Mapping, Optional, Sequence
 
 import numpy as np
 import torch
 
 from .. import ops
+from ..ops.logit_controls import biases_by_token
 
 
 @dataclass(frozen=True)
 class RequestControls:
     """``repetition_penalty`` (positive): logits of tokens that stand in the prompt or the answer are divided by it where they are positive and
     multiplied where not.  ``frequency_penalty`` times the times a token stands in the answer, and ``presence_penalty`` where it stands
-    there at all, are taken off.  ``logit_bias``: token -> what is added to its logit.  ``allowed_tokens``: a function of the list of tokens
-    generated so far that gives the tokens allowed next, as ids or as truth values for the whole vocabulary, or None where all are."""
+    there at all, are taken off.  ``logit_bias``: token (a whole number, or the text of one) -> what is added to its logit.
+    ``allowed_tokens``: a function of the list of tokens generated so far that gives the tokens allowed next, as ids or as truth values for the
+    whole vocabulary, or None where all are."""
     repetition_penalty: float = 1.0
     presence_penalty: float = 0.0
     frequency_penalty: float = 0.0
@@ -29,17 +31,19 @@ class RequestControls:
     allowed_tokens: Optional[Callable[[List[int]], object]] = None
 
     def check(self, vocab: int) -> "RequestControls":
+        """The same with the biases by whole numbers, in a mapping of its own; raises ValueError for what cannot be meant."""
         if not (math.isfinite(self.repetition_penalty) and self.repetition_penalty > 0):
             raise ValueError(f"a repetition penalty is a positive number (1: none), not {self.repetition_penalty}")
         for name in ("presence_penalty", "frequency_penalty"):
             if not math.isfinite(getattr(self, name)):
                 raise ValueError(f"{name} must be a finite number, not {getattr(self, name)}")
-        for token, value in (self.logit_bias or {}).items():
-            if not 0 <= int(token) < vocab or math.isnan(value):
-                raise ValueError(f"a bias of {value} for token {token}: tokens are 0 to {vocab - 1}, biases numbers")
+        biases = biases_by_token(self.logit_bias or {}, vocab)
+        for token, value in biases.items():
+            if math.isnan(value):
+                raise ValueError(f"a bias of {value} for token {token}: biases are numbers")
         if self.allowed_tokens is not None and not callable(self.allowed_tokens):
             raise ValueError("allowed_tokens is a function of the tokens generated so far")
-        return self
+        return replace(self, logit_bias=biases or None)
 
     @property
     def penalises(self) -> bool:
