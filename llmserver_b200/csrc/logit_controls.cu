@@ -19,7 +19,7 @@
 // that overflows is not used: marks are then worked out in the walk.
 //
 // Sampling (sampling.cu's rule) takes the controlled logits as they are made, without writing them.  A second kernel picks the best
-// slice of a row, gives -1 where nothing is left to draw from, and writes the token behind the request's history: all histories have
+// slice of a row, gives -1 where a row's controls leave nothing to draw from, and writes the token behind the request's history: all histories have
 // been read by then, whatever rows share one.
 //
 // What bounds it: the logits, read once (and written once by the form that returns them), and behind that the block's phases, which all blocks go
@@ -414,6 +414,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* 
     }
 }
 
+// Whether anything is said about a row (an index that names nothing says nothing).
+__device__ __forceinline__ bool any_controls(const Controls& c, int row) {
+    auto names = [&](const int* rows, int count) { return rows != nullptr && rows[row] >= 0 && rows[row] < count; };
+    return (c.penalties != nullptr && names(c.history_rows, c.histories)) || names(c.bias_rows, c.bias_lists) || names(c.mask_rows, c.mask_count);
+}
+
 // One warp per row.
 __global__ void control_pick_kernel(const float* __restrict__ partial_scores, const int* __restrict__ partial_indices, int slices,
                                     int* __restrict__ out, int* history, const Controls c, int note, const int* __restrict__ flag_a,
@@ -431,7 +437,8 @@ __global__ void control_pick_kernel(const float* __restrict__ partial_scores, co
         const int other_index = __shfl_xor_sync(0xffffffffu, best_index, offset);
         take_better(best, best_index, other, other_index);
     }
-    const int token = best == -INFINITY ? -1 : best_index;
+    // (a row of which nothing is said: as sampling.cu has it, whoever shares the step)
+    const int token = best != -INFINITY ? best_index : any_controls(c, row) ? -1 : 0;
     if (note) {
         const int at = c.history_rows[row], place = c.lengths[row];
         // of rows with one place the last has it

@@ -1,16 +1,20 @@
 """Requests' controls through the engine beside what can go wrong in a step, on the device."""
+import math
+
 import pytest
 import torch
 
 from dikusun_configs import DIKUSUN
+from llmserver_b200 import ops
 from llmserver_b200.engine.engine import Engine
 from test_gpu_kernels import DEVICE
+from test_gpu_logit_controls import Request as Row
+from test_gpu_logit_controls import controls_of, finished, logits_for
 
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("cuda_graphs", [False, True])
-@pytest.mark.parametrize("name", ["gla_only", "all_kinds"])
+@pytest.mark.parametrize("name,cuda_graphs", [("gla_only", False), ("all_kinds", False), ("all_kinds", True)])
 def test_a_grammar_that_raises_leaves_no_token_in_a_recurrent_state(name, cuda_graphs):
     """The step is run again: the answers of every request in it are those of a run in which nothing raised (the 32-bit path gives the
     same logits whatever else a step holds)."""
@@ -43,3 +47,30 @@ def test_a_grammar_that_raises_leaves_no_token_in_a_recurrent_state(name, cuda_g
         return [request.generated_token_ids for request in requests]
 
     assert run((0, 1, 2, 7, 11)) == run(())
+
+
+@pytest.mark.parametrize("vocab", [700, 3000, 50000])
+@pytest.mark.parametrize("warm", [False, True])
+def test_a_row_without_controls_draws_as_it_would_alone(vocab, warm):
+    """Logits that are all NaN, all -inf or partly so, beside rows that are steered."""
+    logits = logits_for(8, vocab, 40)
+    logits[1], logits[2] = math.nan, -math.inf
+    logits[3, ::2], logits[3, 1::2] = math.nan, -math.inf
+    logits[4] = math.inf
+    logits[5, 9:] = -math.inf
+    none = torch.zeros(vocab, dtype=torch.bool)
+    requests = [Row([1, 2], [3], 1.5, 0.5, 0.5), Row(), Row(), Row(), Row(), Row(), Row(allowed=none), Row(bias={4: 1.0})]
+    controls = controls_of(requests, vocab)
+    for row in range(1, 6):
+        controls.history_rows[row] = -1
+    drawn = (torch.full((8,), 0.7, device=DEVICE), torch.arange(8, device=DEVICE), torch.arange(8, dtype=torch.int32, device=DEVICE)) if warm else ()
+    for note in (False, True):
+        got = ops.sample(logits, *drawn, controls=controls, note=note)
+        finished()
+        alone = [int(ops.sample(logits[row:row + 1], *(part[row:row + 1] for part in drawn))) for row in range(8)]
+        assert got.tolist()[1:6] == alone[1:6] and int(got[6]) == -1
+    # controls that say something leave nothing of such a row
+    controls.history_rows[1:4] = controls.history_rows[0]
+    got = ops.sample(logits, *drawn, controls=controls)
+    finished()
+    assert got.tolist()[1:4] == [-1, -1, -1]
