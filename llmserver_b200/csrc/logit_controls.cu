@@ -437,8 +437,11 @@ __global__ void control_pick_kernel(const float* __restrict__ partial_scores, co
         const int other_index = __shfl_xor_sync(0xffffffffu, best_index, offset);
         take_better(best, best_index, other, other_index);
     }
-    // (a row of which nothing is said: as sampling.cu has it, whoever shares the step)
-    const int token = best != -INFINITY ? best_index : any_controls(c, row) ? -1 : 0;
+    int token = best_index;
+    if (best == -INFINITY) {      // a quotient may be too large for 32 bits: the token is then still one that is left
+        if (!any_controls(c, row)) token = 0;      // as sampling.cu has it, whoever shares the step
+        else if (best_index == 0x7fffffff) token = -1;
+    }
     if (note) {
         const int at = c.history_rows[row], place = c.lengths[row];
         // of rows with one place the last has it

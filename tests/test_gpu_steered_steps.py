@@ -74,3 +74,16 @@ def test_a_row_without_controls_draws_as_it_would_alone(vocab, warm):
     got = ops.sample(logits, *drawn, controls=controls)
     finished()
     assert got.tolist()[1:4] == [-1, -1, -1]
+
+
+def test_a_score_that_32_bits_cannot_hold_is_still_a_token():
+    """A temperature below the normal numbers makes every quotient -inf: the lowest of the tokens that the mask leaves."""
+    vocab = 5000
+    logits = -1 - logits_for(3, vocab, 41).abs()
+    few = torch.zeros(vocab, dtype=torch.bool)
+    few[[37, 4100]] = True
+    controls = controls_of([Row(allowed=few), Row([1], [], 1.5), Row(allowed=few & False)], vocab)
+    for temperature in (1e-39, 2e-39):
+        got = ops.sample(logits, torch.full((3,), temperature, device=DEVICE), torch.arange(3, device=DEVICE), torch.zeros(3, dtype=torch.int32, device=DEVICE), controls=controls)
+        finished()
+        assert got.tolist() == [37, 0, -1]
