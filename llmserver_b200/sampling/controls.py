@@ -17,6 +17,11 @@ from .. import ops
 from ..ops.logit_controls import biases_by_token
 
 
+def _in_32_bits(value: float) -> float:
+    with np.errstate(over="ignore"):
+        return float(np.float32(value))
+
+
 @dataclass(frozen=True)
 class RequestControls:
     """``repetition_penalty`` (positive): logits of tokens that stand in the prompt or the answer are divided by it where they are positive and
@@ -32,11 +37,12 @@ class RequestControls:
 
     def check(self, vocab: int) -> "RequestControls":
         """The same with the biases by whole numbers, in a mapping of its own; raises ValueError for what cannot be meant."""
-        if not (math.isfinite(self.repetition_penalty) and self.repetition_penalty > 0):
-            raise ValueError(f"a repetition penalty is a positive number (1: none), not {self.repetition_penalty}")
+        # (as the device holds them)
+        if not (math.isfinite(_in_32_bits(self.repetition_penalty)) and _in_32_bits(self.repetition_penalty) > 0):
+            raise ValueError(f"a repetition penalty is a positive number of 32 bits (1: none), not {self.repetition_penalty}")
         for name in ("presence_penalty", "frequency_penalty"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} must be a finite number, not {getattr(self, name)}")
+            if not math.isfinite(_in_32_bits(getattr(self, name))):
+                raise ValueError(f"{name} must be a finite number of 32 bits, not {getattr(self, name)}")
         biases = biases_by_token(self.logit_bias or {}, vocab)
         for token, value in biases.items():
             if math.isnan(value):

@@ -39,3 +39,19 @@ def test_a_request_keeps_the_biases_it_came_with():
     biases[VOCAB + 5] = 2.0
     del biases[3]
     assert request.controls.logit_bias == {3: 1.0}
+
+
+@pytest.mark.parametrize("given,message", [({"repetition_penalty": 1e-46}, "positive"), ({"repetition_penalty": 1e39}, "positive"), ({"presence_penalty": 1e300}, "finite"),
+                                           ({"presence_penalty": -1e39}, "finite"), ({"frequency_penalty": 3.5e38}, "finite")])
+def test_what_32_bits_cannot_hold_is_refused(given, message):
+    """The device holds penalties in 32 bits, where these are zero or infinite."""
+    with pytest.raises(ValueError, match=message):
+        RequestControls(**given).check(50)
+
+
+def test_what_32_bits_can_hold_is_taken():
+    for given in ({"repetition_penalty": 1e-45}, {"repetition_penalty": 3.4e38}, {"presence_penalty": -3.4e38}, {"frequency_penalty": 1e-300}):
+        RequestControls(**given).check(50)
+    # a bias may be infinite, and one beyond 32 bits is that
+    biases = RequestControls(logit_bias={3: float("-inf"), 4: -1e300}).check(50).logit_bias
+    assert ops.bias_lists([biases], 50, "cpu")["bias_values"].tolist() == [-float("inf")] * 2
