@@ -90,8 +90,9 @@ class Engine:
                     max_new_tokens: Optional[int] = None, temperature: float = 0.0, seed: Optional[int] = None,
                     ignore_eos: Optional[bool] = None, **controls) -> Request:
         """Queues a request.  ``controls``: ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` and
-        ``allowed_tokens`` (see ``sampling.RequestControls``); a request whose controls leave no token to draw ends with the reason
-        "error".  ``prompt`` exists for signature parity with the reference
+        ``allowed_tokens`` (see ``sampling.RequestControls``); a request whose controls leave no token to draw, or whose ``allowed_tokens`` gives
+        what is no token (``request.error`` then says so), ends with the reason "error".  What ``allowed_tokens`` raises comes out of ``step``, which
+        has not run and may be called again.  ``prompt`` exists for signature parity with the reference
         (utils/engine.py:210) and must be None or a sequence of ids: text needs a tokenizer, which
         this engine does not have."""
         if prompt_token_ids is None:

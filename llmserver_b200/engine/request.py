@@ -55,6 +55,7 @@ class Request:
         self.max_new_tokens = max_new_tokens
         self.temperature, self.seed, self.ignore_eos = float(temperature), int(seed), ignore_eos
         self.controls = controls          # sampling.RequestControls, or None
+        self.error: Optional[str] = None  # what was wrong with its controls, where they ended it with the reason "error"
         self.status = RequestStatus.WAITING
         self.finish_reason: Optional[RequestFinishReason] = None
         self.num_computed_tokens = 0      # tokens of ``feed`` whose keys and values are in the cache

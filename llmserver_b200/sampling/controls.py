@@ -68,6 +68,8 @@ def mask_words(allowed, vocab: int) -> np.ndarray:
         if given.shape != (vocab,):
             raise ValueError(f"truth values for {given.shape} tokens, the vocabulary has {vocab}")
         given = np.nonzero(given)[0]
+    if given.size and (given.dtype.kind not in "iuf" or (given.dtype.kind == "f" and not (given == np.floor(given)).all())):
+        raise ValueError(f"allowed tokens are whole numbers, not {given.reshape(-1)[0]!r} and the like")
     given = given.reshape(-1).astype(np.int64) if given.size else np.zeros(0, dtype=np.int64)
     if given.size and (given.min() < 0 or given.max() >= vocab):
         raise ValueError(f"an allowed token is outside the vocabulary of {vocab}")
@@ -112,7 +114,8 @@ class ControlTable:
 
     def allowed(self, requests: Sequence) -> List[Optional[np.ndarray]]:
         """Asks the grammars of a step's rows: per row the words of its mask, or None where all tokens are allowed.  What a grammar raises goes on
-        to the caller with a note that names the request; nothing has changed here by then."""
+        to the caller with a note that names the request; nothing has changed here by then.  A grammar that gives what is no token leaves its
+        request nothing to draw from, and ``request.error`` says why."""
         found: List[Optional[np.ndarray]] = []
         for request in requests:
             words = None
@@ -122,7 +125,11 @@ class ControlTable:
                 except Exception as error:
                     error.add_note(f"raised by allowed_tokens of request {request.request_id!r}")
                     raise
-                words = None if given is None else mask_words(given, self.vocab)
+                try:
+                    words = None if given is None else mask_words(given, self.vocab)
+                except (TypeError, ValueError) as error:      # no mask can be made of it: the request ends, the others go on
+                    request.error = f"allowed_tokens: {error}"
+                    words = np.zeros(-(-self.vocab // 32), dtype=np.int32)
             found.append(words)
         return found
 

@@ -128,3 +128,29 @@ def test_the_request_whose_grammar_raises_can_be_cancelled(monkeypatch, replayed
         pass
     assert bad.finish_reason is RequestFinishReason.CANCELLED and bad.generated_token_ids == answer(PROMPTS[0], 4)
     assert good.generated_token_ids == answer(PROMPTS[1], 8)
+
+
+@pytest.mark.parametrize("replayed", [False, True])
+@pytest.mark.parametrize("given,said", [([1, VOCAB], "outside"), ([-1], "outside"), (torch.ones(VOCAB + 1, dtype=torch.bool), "truth values"), ([1.5], "whole"), (7, "iterable"),
+                                        (["a"], "whole"), ([1 << 70], "whole")])
+def test_a_request_whose_grammar_gives_what_is_no_token_ends_alone(monkeypatch, replayed, given, said):
+    model = SummingModel()
+    engine = engine_of(model, monkeypatch, replayed)
+    bad = engine.add_request(prompt_token_ids=PROMPTS[0], allowed_tokens=lambda sofar: given if len(sofar) == 5 else None)
+    others = [engine.add_request(prompt_token_ids=PROMPTS[1], frequency_penalty=0.0, logit_bias={0: 0.0}), engine.add_request(prompt_token_ids=PROMPTS[2])]
+    while engine.step():
+        pass
+    assert bad.finish_reason is RequestFinishReason.ERROR and bad.generated_token_ids == answer(PROMPTS[0], 5) and said in bad.error
+    for request, prompt in zip(others, PROMPTS[1:]):
+        assert request.finish_reason is RequestFinishReason.LENGTH and request.generated_token_ids == answer(prompt, 8) and request.error is None
+    assert not engine.cache.requests
+
+
+def test_masks_take_whole_numbers_only():
+    from llmserver_b200.sampling.controls import mask_words
+    import numpy as np
+    for given in ([2.0, 5.0], np.array([2, 5], dtype=np.uint8), torch.tensor([5, 2], dtype=torch.int32), (2, 5), {2: "a", 5: "b"}, torch.tensor([[2], [5]])):
+        assert mask_words(given, 40).tolist() == [(1 << 2) | (1 << 5), 0]
+    for wrong in ([2.5], [float("nan")], [None], ["2"], [1 + 2j]):
+        with pytest.raises(ValueError, match="whole"):
+            mask_words(wrong, 40)
