@@ -76,6 +76,8 @@ def _checked(operand: BlockScaled, block_rows: int, name: str) -> BlockScaled:
     values, scales = operand.values, operand.scales
     if not (values.is_cuda and scales.is_cuda):
         raise KernelError(f"{name} must live on a CUDA device (there is no CPU path); it is on {values.device} and {scales.device}")
+    if values.device != scales.device:
+        raise KernelError(f"{name}: values and scales lie on {values.device} and {scales.device}")
     if values.dtype != FLOAT8 or scales.dtype != torch.float32 or values.dim() != 2:
         raise KernelError(f"{name} must be float8_e4m3fn [rows, columns] with float32 scales, got {values.dtype} {tuple(values.shape)} and {scales.dtype}")
     if operand.block_rows != block_rows:
