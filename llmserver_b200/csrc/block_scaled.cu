@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) quantize_matrix_kernel(const T* __re
 // pitch a multiple of 16 and at least inner, out 16-byte aligned.
 LLM_EXPORT int llm_quantize_blocks(const void* x, int dtype, void* out, float* scales, int rows, int inner, long long pitch, int block_rows,
                                    cudaStream_t stream) {
-    if (rows < 0 || inner < 1 || pitch < inner || pitch % 16 != 0 || !aligned16(out) || (block_rows != 1 && block_rows != kBlock)) {
+    if (rows < 0 || rows > kMostAlong || inner < 1 || inner > kMostAlong || pitch < inner || pitch % 16 != 0 || !aligned16(out) || (block_rows != 1 && block_rows != kBlock)) {
         llm_set_error("quantize_blocks: %d rows of %d (pitch %lld) in blocks of %d rows", rows, inner, pitch, block_rows);
         return LLM_REFUSED;
     }

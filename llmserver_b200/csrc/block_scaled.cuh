@@ -6,6 +6,7 @@
 namespace block_scaled {
 
 constexpr int kBlock = 128;              // numbers along a row that share a scale
+constexpr int kMostAlong = 0x7fffff00;   // rows or columns: places are counted in 32 bits, up to the end of a tile
 
 // The scale of a block whose largest magnitude has the bits `largest`, and its inverse: the exponent of the magnitude, one more where the
 // mantissa is above 448's (0x600000), less 8; not below 2^-126.  NaN where the block holds an infinity or a NaN.

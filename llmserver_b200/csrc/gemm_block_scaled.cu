@@ -324,7 +324,7 @@ int launch_block_scaled(const void* x, long long x_pitch, const void* w, long lo
 }
 
 int refuse_product(long long m, int n, int inner, long long x_pitch, long long w_pitch) {
-    if (m < 0 || n < 1 || inner < 1 || x_pitch < inner || x_pitch % 16 != 0 || w_pitch < inner || w_pitch % 16 != 0 || m > 65535 * 128LL ||
+    if (m < 0 || n < 1 || n > kMostAlong || inner < 1 || inner > kMostAlong || x_pitch < inner || x_pitch % 16 != 0 || w_pitch < inner || w_pitch % 16 != 0 || m > 65535 * 128LL ||
         (m + 127) / 128 * ((n + 127LL) / 128) * ((inner + 127LL) / 128) > 0x7fffffffLL / kMaxSplit) {
         llm_set_error("block_linear: [%lld, %d] x [%d, %d]^T with rows %lld and %lld bytes apart is not supported", m, inner, n, inner, x_pitch, w_pitch);
         return LLM_REFUSED;

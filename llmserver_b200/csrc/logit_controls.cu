@@ -58,6 +58,7 @@ constexpr int kListed = 2048;           // marked tokens of a slice that are wor
 constexpr int kMostShared = 68 << 10;   // of a block
 constexpr int kLeastSlice = 2048;       // tokens
 constexpr int kListByScan = 8 * kThreads;      // slices of so many tokens and fewer are marked first and looked through for marks afterwards
+constexpr int kMostVocab = 0x7ffe0000;  // places are counted in 32 bits, up to a slice and a lap behind the last
 constexpr int kBadRow = 8;              // error code: a row names a history, list or mask that does not exist
 
 // What a block needs of its row.
@@ -477,8 +478,8 @@ int slice_of(int rows, int vocab, bool small) {
     }
 }
 int refuse_controls(const char* what, const Controls& c, int rows, int vocab) {
-    if (rows < 0 || rows > 65535 || vocab < 1) {
-        llm_set_error("%s: %d rows of %d logits (1 to 65535 rows per launch)", what, rows, vocab);
+    if (rows < 0 || rows > 65535 || vocab < 1 || vocab > kMostVocab) {
+        llm_set_error("%s: %d rows of %d logits (1 to 65535 rows per launch, of 1 to %d)", what, rows, vocab, kMostVocab);
         return LLM_REFUSED;
     }
     if (c.masks != nullptr && c.mask_words < (vocab + 31) / 32) {

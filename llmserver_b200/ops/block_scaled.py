@@ -19,6 +19,7 @@ import torch
 from .library import KernelError, call, check, current_device, dtype_code, stream_handle, wait_error_flag
 
 BLOCK = 128
+MOST_ALONG = 0x7FFFFF00     # rows or columns: the kernels count places in 32 bits
 FLOAT8 = torch.float8_e4m3fn
 
 
@@ -119,8 +120,10 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1) -> BlockScaled:
         raise KernelError(f"quantize_blocks takes a matrix, got {tuple(x.shape)}")
     if block_rows not in (1, BLOCK):
         raise KernelError(f"blocks have 1 or {BLOCK} rows, not {block_rows}")
-    current_device(x, "x")
     rows, columns = x.shape
+    if max(rows, columns) > MOST_ALONG:
+        raise KernelError(f"quantize_blocks takes at most {MOST_ALONG} rows and columns, got {rows} and {columns}")
+    current_device(x, "x")
     pitch = _pitch(columns)
     values = x.new_empty((rows, pitch), dtype=FLOAT8)
     scales = x.new_empty((_blocks(rows, block_rows), _blocks(columns)), dtype=torch.float32)
@@ -148,6 +151,8 @@ def block_linear(x, weight: BlockScaled, out: Optional[torch.Tensor] = None, out
     rows, columns = held.shape
     if columns != inner:
         raise KernelError(f"x has {columns} columns, the weight {inner}")
+    if max(rows, inner, cols) > MOST_ALONG:
+        raise KernelError(f"block_linear takes at most {MOST_ALONG} rows and columns, got {rows} rows and a weight [{cols}, {inner}]")
     index = values.get_device()
     if held.get_device() != index or (out is not None and out.get_device() != index):
         raise KernelError(f"the operands lie on {held.device} and {values.device}" + ("" if out is None else f", the output on {out.device}"))

@@ -48,6 +48,7 @@ class LogitControls:
 # values and rows of the biases, how many lists and entries; masks, mask_rows, how many masks and words; the error flag
 _DESCRIPTION = struct.Struct("@PPPPPiiPPPPiiPPiiP")
 _LEAST_SLICE = 2048        # a row is scanned in no more slices than of so many tokens
+MOST_LOGITS = 0x7FFE0000   # rows or tokens: the kernels count places in 32 bits
 MOST_HISTORY = (1 << 30) - 1        # tokens of a request that a 30-bit count can hold
 
 
@@ -68,8 +69,10 @@ def _described(logits: torch.Tensor, controls: LogitControls, note: bool = False
     check(logits, "logits", torch.float32)
     if logits.dim() != 2:
         raise KernelError(f"logits must be [rows, vocabulary], got {tuple(logits.shape)}")
-    current_device(logits, "logits")
     rows, vocab = logits.shape
+    if max(rows, vocab) > MOST_LOGITS:
+        raise KernelError(f"logits of at most {MOST_LOGITS} rows and tokens, got {rows} and {vocab}")
+    current_device(logits, "logits")
     index, whole = logits.get_device(), torch.int32
     c = controls
     history = lengths = prompts = history_rows = penalties = histories = capacity = 0
@@ -105,6 +108,8 @@ def _described(logits: torch.Tensor, controls: LogitControls, note: bool = False
                 or bits.shape[1] * 32 < vocab or not plain(c.mask_rows, whole, row)):
             _complaint(logits, c)
         masks, (mask_count, words), mask_rows = bits.data_ptr(), bits.shape, c.mask_rows.data_ptr()
+    if max(histories, lists, entries, mask_count, words) >= 1 << 31:
+        raise KernelError(f"the controls hold {histories} histories, {lists} lists of {entries} biases and {mask_count} masks of {words} words; 32 bits count them")
     return _DESCRIPTION.pack(penalties, history, history_rows, lengths, prompts, histories, capacity, starts, ids, values, bias_rows, lists, entries,
                              masks, mask_rows, mask_count, words, wait_error_flag(logits.device).data_ptr())
 

@@ -62,3 +62,43 @@ def test_both_looks_at_an_operand_agree(block_rows):
         assert not _sound(made, block_rows)
         with pytest.raises(KernelError):
             _checked(made, block_rows, "x")
+
+
+def claimed(shape, dtype, strides=None):
+    """One of any size, without memory."""
+    if strides is None:
+        return Claimed(torch.empty(shape, dtype=dtype, device="meta"), 0)
+    return Claimed(torch.empty_strided(shape, strides, dtype=dtype, device="meta"), 0)
+
+
+HUGE = (1 << 32) + 3      # 3, where 32 bits are kept of it
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """They do not reach a launcher, whose whole numbers are of 32 bits."""
+    for shape in ((HUGE, 1), (1, HUGE), ((1 << 31) - 1, 1), (1, (1 << 31) - 1)):
+        with pytest.raises(KernelError, match="at most"):
+            ops.quantize_blocks(claimed(shape, torch.bfloat16))
+        with pytest.raises(KernelError, match="at most"):
+            ops.control_logits(claimed(shape, torch.float32), ops.LogitControls())
+        with pytest.raises(KernelError, match="at most"):
+            ops.sample(claimed(shape, torch.float32), controls=ops.LogitControls())
+    for rows, inner, cols in ((HUGE, 16, 16), (16, HUGE, 16), (16, 16, HUGE)):
+        pitch = -(-inner // 16) * 16
+        weight = ops.BlockScaled(claimed((cols, inner), F8, (pitch, 1)), claimed((-(-cols // 128), -(-inner // 128)), torch.float32))
+        with pytest.raises(KernelError, match="at most"):
+            ops.block_linear(claimed((rows, inner), torch.bfloat16), weight)
+
+
+def test_launchers_refuse_places_that_32_bits_cannot_count():
+    library, most = ops.library(), (1 << 31) - 1
+    pitch = 1 << 31
+    assert library.llm_quantize_blocks(0, 0, 0, 0, 1, most, pitch, 1, 0) == -1
+    assert library.llm_quantize_blocks(0, 0, 0, 0, most, 16, 16, 1, 0) == -1
+    for n, inner in ((most, 16), (16, most)):
+        assert library.llm_block_linear(0, -1, pitch, 0, 0, pitch, 0, 0, 0, 1, n, inner, 0, 0, 0) == -1
+    from llmserver_b200.ops.logit_controls import _DESCRIPTION
+    said = _DESCRIPTION.pack(*[0] * 18)
+    assert library.llm_control_logits(0, 0, 1, most, said, 0) == -1
+    assert library.llm_control_sample(0, 0, 0, 0, 0, 1, most, said, 0, 0, 0, 0, 0, 0) == -1
+    assert library.llm_control_logits(0, 0, 0, 0x7FFE0000, said, 0) == 0 and library.llm_block_linear(0, -1, pitch, 0, 0, pitch, 0, 0, 0, 0, 0x7FFFFF00, 16, 0, 0, 0) == 0
