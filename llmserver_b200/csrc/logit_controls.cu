@@ -78,8 +78,9 @@ __device__ __forceinline__ RowControls controls_of(const Controls& c, int row) {
     int at = -1, list = -1, mask = -1, length = 0, prompt = 0;
     RowControls r = {};
     r.repetition = 1.0f;
+    if (c.history_rows != nullptr) at = c.history_rows[row];      // also where tokens are only noted there: a bad one is reported here, so that
+                                                                   // the flag is settled when control_pick_kernel hands it on
     if (c.penalties != nullptr) {
-        at = c.history_rows[row];
         length = c.lengths[row];
         prompt = c.prompt_lengths[row];
         r.repetition = c.penalties[3 * (size_t)row];
@@ -450,7 +451,6 @@ __global__ void control_pick_kernel(const float* __restrict__ partial_scores, co
         for (int other = row + 1 + lane; other < (int)gridDim.x; other += 32)
             if (c.history_rows[other] == at && c.lengths[other] == place) last = false;
         last = __all_sync(0xffffffffu, last);
-        if (lane == 0 && at >= c.histories && c.error_flag != nullptr) atomicExch(c.error_flag, kBadRow);
         if (lane == 0 && last && token >= 0 && at >= 0 && at < c.histories && place >= 0 && place < c.capacity)
             history[(size_t)at * c.capacity + place] = token;
     }

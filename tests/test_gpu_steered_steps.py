@@ -87,3 +87,29 @@ def test_a_score_that_32_bits_cannot_hold_is_still_a_token():
         got = ops.sample(logits, torch.full((3,), temperature, device=DEVICE), torch.arange(3, device=DEVICE), torch.zeros(3, dtype=torch.int32, device=DEVICE), controls=controls)
         finished()
         assert got.tolist() == [37, 0, -1]
+
+
+def test_a_history_that_does_not_exist_is_reported_with_the_step():
+    """The flag behind the tokens is that of this step, whichever row is at fault, and with penalties or without."""
+    from llmserver_b200.ops.library import KernelError, check_wait_errors, wait_error_flag
+    vocab, rows = 300, 400
+    logits = logits_for(rows, vocab, 42)
+    controls = controls_of([Row([row % vocab], [], 1.2) for row in range(rows)], vocab, capacity=6)
+    flag, own = wait_error_flag(torch.device(DEVICE)), torch.full((1,), 5, dtype=torch.int32, device=DEVICE)
+    good = controls.history_rows.clone()
+    for penalties in (controls.penalties, None):
+        controls.penalties = penalties
+        for bad in (0, 1, rows - 1):
+            controls.history_rows.copy_(good)
+            controls.history_rows[bad] = rows + 2
+            for note in (True, False):
+                got = ops.sample(logits, controls=controls, flags=(own, flag), note=note)
+                torch.cuda.synchronize()
+                assert got.tolist()[rows:] == [5, 8]
+                with pytest.raises(KernelError, match="does not exist"):
+                    check_wait_errors()
+            ops.control_logits(logits, controls)
+            torch.cuda.synchronize()
+            with pytest.raises(KernelError, match="does not exist"):
+                check_wait_errors()
+    finished()
