@@ -218,7 +218,8 @@ __device__ __forceinline__ int ordered(float v) {
 __device__ __forceinline__ float unordered(int v) { return __int_as_float(v >= 0 ? v : v ^ 0x7fffffff); }
 
 // The draw of a row at a temperature.  Most tokens cannot win, and an upper bound of their score says so for a fifth of its price: with
-// u = 1 - v, -log u >= v, so that the noise -log(-log u) is at most -log v, which is below 17.  The bound's own errors (the approximate logarithm's,
+// -log u >= 1 - u > v, the noise -log(-log u) is below -log v (v is 0 for the last of the words, and the bound infinite); the noise itself, with
+// u at most 1 - 2^-24, is below 17.  The bound's own errors (the approximate logarithm's,
 // the product's for the quotient) are below a thousandth and a millionth of the quotient, and a quotient that needs noise to reach a score is within 17 of
 // it: the score is lowered by as much, once for many tokens.
 struct Draw {
@@ -286,18 +287,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* 
     __syncthreads();
 
     const bool apart = r.marks && n_listed <= kListed, inside = r.marks && !apart;      // where what is marked is worked out
-    float best = -INFINITY, listed_logits[SAMPLE ? 1 : kListed / kThreads];
+    float best = -INFINITY;
     int best_index = 0x7fffffff;
-    // Logits that are returned into their own place are read before the walk writes there; others behind it, from L2: in front of it they waited
-    // for memory behind the walks of other blocks.
-    const bool in_place = !SAMPLE && logits == out;
-    if (apart && in_place) {
-#pragma unroll
-        for (int k = 0; k < kListed / kThreads; ++k) {
-            const int e = threadIdx.x + k * kThreads;
-            listed_logits[SAMPLE ? 0 : k] = e < n_listed ? src[begin + listed[e]] : 0.0f;
-        }
-    }
     constexpr int kEach = FOUR ? 4 : 1, kGroups = kAhead / kEach;      // tokens that lie side by side, groups of them
     for (int lap = 0; lap < count; lap += kAhead * kThreads) {
         auto place = [&](int a) { return lap + (a / kEach * kThreads + (int)threadIdx.x) * kEach + a % kEach; };
@@ -376,13 +367,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm) control_kernel(const float* 
         }
     }
     if (apart) {
-        if (!SAMPLE) __syncthreads();      // the walk has written what stood there
+        // Behind the walk these logits come from L2 (in front of it they waited for memory behind the walks of other blocks).  Where the result goes
+        // to the logits' own place the walk has written each back as it was, or -inf where the mask bans it, which it then stays.
+        if (!SAMPLE) __syncthreads();
 #pragma unroll
         for (int k = 0; k < kListed / kThreads; ++k) {
             const int e = threadIdx.x + k * kThreads;
             if (e >= n_listed) break;
             const int place = listed[e], i = begin + place;
-            float logit = controlled<SMALL>(r, in_place ? listed_logits[SAMPLE ? 0 : k] : src[i], marks.of(place), i);
+            float logit = controlled<SMALL>(r, src[i], marks.of(place), i);
             if (r.mask != nullptr && (allowed[place >> 5] >> (i & 31) & 1u) == 0) logit = -INFINITY;
             if (!SAMPLE) dst[i] = logit;
             else if (logit > -INFINITY) take_better(best, best_index, warm ? draw.score(logit, i) : logit, i);
