@@ -154,3 +154,14 @@ def test_masks_take_whole_numbers_only():
     for wrong in ([2.5], [float("nan")], [None], ["2"], [1 + 2j]):
         with pytest.raises(ValueError, match="whole"):
             mask_words(wrong, 40)
+
+
+@pytest.mark.parametrize("replayed", [False, True])
+@pytest.mark.parametrize("none", [[], torch.zeros(VOCAB, dtype=torch.bool), range(0)])
+def test_a_request_with_nothing_left_keeps_what_it_has_drawn(monkeypatch, replayed, none):
+    engine = engine_of(SummingModel(), monkeypatch, replayed)
+    stuck, other = engine.add_request(prompt_token_ids=PROMPTS[0], allowed_tokens=lambda sofar: none if len(sofar) == 3 else None), engine.add_request(prompt_token_ids=PROMPTS[1])
+    while engine.step():
+        pass
+    assert stuck.finish_reason is RequestFinishReason.ERROR and stuck.generated_token_ids == answer(PROMPTS[0], 3) and stuck.error is None
+    assert other.finish_reason is RequestFinishReason.LENGTH and other.generated_token_ids == answer(PROMPTS[1], 8)
