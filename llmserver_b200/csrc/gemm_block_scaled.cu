@@ -10,8 +10,8 @@
 // that do not exist.  A stage of the ring is one block of 128 along k: 16 KiB of W and 2 to 8 KiB of x, which are one swizzle atom wide.  The MMAs of a block go to one of several
 // buffers of tensor memory, so that they run ahead of the warps that scale and add.
 //
-// What bounds it: W's bytes.  8 rows by 151936 x 4096 98 us, 6.4 TB/s, 0.97 of a copy; 1 row by 24576 x 4096 20.9 us with the kernel that
-// brings the row to 8 bits, 4.8 TB/s in all, 6.1 once the rings are full.
+// What bounds it: W's bytes.  8 rows by 151936 x 4096 98 us, 6.4 TB/s, 0.97 of a copy; 1 row by 24576 x 4096 20.3 us with the kernel that
+// brings the row to 8 bits, 5.0 TB/s in all, 6.1 once the rings are full.
 //
 // Where tiles do not come out even on the SMs, k is split over a cluster and the parts are added through distributed shared memory in
 // the order of k (see split_of).

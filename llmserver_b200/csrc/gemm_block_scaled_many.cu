@@ -17,7 +17,8 @@
 // What bounds it, in SM cycles for a unit of 128 x 256: the MMAs alone 513, with copies, waits and signals 540, with the adders' reads and 32768
 // products and sums 670 in a loop of nothing else; this kernel 800.  Counted in time the power limit comes first: with random operands the SMs run
 // at 1.3 to 1.4 GHz, and even the MMAs with their copies alone take 422 ns of the 580 of a unit.
-// 8192 x 4096 -> 24576: 745 us behind 8-bit rows, 2210 TFLOP/s; 500 x 4096 -> 4096: 13.1 us; 100 x 4096 -> 24576: 22.0 us, 4.5 TB/s.
+// Behind 8-bit rows, over fresh operands for two seconds on end (and in a burst of a few milliseconds, before the power limit holds the clock down):
+// 8192 x 4096 -> 24576 856 us, 1926 TFLOP/s (756); 500 x 4096 -> 4096 14.0 us (12.8); 100 x 4096 -> 24576 24.3 us, W at 4.1 TB/s (22.3).
 // Sixteen adders of half the columns take 830 to 1050 cycles, reads of 16 columns at a time 980, and sums kept as single numbers 1440 (they spill).
 //
 // Roles, bounded waits and the treatment of ragged sizes are those of gemm_block_scaled.cu.

@@ -23,8 +23,9 @@
 // been read by then, whatever rows share one.
 //
 // What bounds it: the logits, read once (and written once by the form that returns them), and behind that the block's phases, which all blocks go
-// through at the same time.  64 rows of 151936 from memory: returned 15.5 us without controls (5 TB/s) and 24.6 with histories of 4096 tokens, 50 biases
-// and masks; drawn greedily 15.3 and 22.5, at temperatures 24.3 and 30.0 (20 instructions a token for its random word and the bound).  1 row 4.8 and 8.7.
+// through at the same time.  In a graph of such steps over logits from memory, 64 rows of 151936: returned 15.6 us without controls (5 TB/s) and 24.7 with
+// histories of 4096 tokens, 50 biases and masks (29.4 call after call); drawn greedily 15.7 and 23.0, at temperatures 24.4 and 30.4 (31.1 call after call; 20
+// instructions a token for its random word and the bound).  1 row and a short history: returned 3.7, drawn 7.7.
 #include "sampling.cuh"
 
 // (the caller fills this in field by field)

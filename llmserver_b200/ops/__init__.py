@@ -174,8 +174,9 @@ def sample(logits: torch.Tensor, temperatures: Optional[torch.Tensor] = None, se
     values follow the tokens; the result is then [R + 2].
 
     ``controls``: the tokens are drawn from ``control_logits(logits, controls)``, which is not written; a row whose controls leave
-    nothing to draw from gets -1.  ``note``: each token drawn is written behind its request's history (history[history_rows[r],
-    lengths[r]], where there is room), after all rows' histories have been read; of rows with one such place the last notes its token."""
+    nothing to draw from (no logit above -inf) gets -1.  ``note``: each token drawn is written behind its request's history (history[history_rows[r],
+    lengths[r]], where there is room), after all rows' histories have been read; of rows with one such place only the last notes, its
+    token or, where it has none, nothing.  A row of which nothing is said (its indices are -1) draws what it would without controls."""
     if controls is not None:
         return sample_controlled(logits, temperatures, seeds, steps, out, flags, controls, note)
     if note:

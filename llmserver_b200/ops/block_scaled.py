@@ -134,7 +134,8 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1) -> BlockScaled:
 
 def block_linear(x, weight: BlockScaled, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y = x W^T for W in 8 bits: what ``ops.linear`` does with a ``BlockScaled`` weight.  ``x`` [N, in]: float32 or bfloat16 (brought to 8
-    bits as ``quantize_blocks`` does), or a ``BlockScaled`` of single rows.  Sums and scales are 32-bit; the result is rounded once to
+    bits as ``quantize_blocks`` does), or a ``BlockScaled`` of single rows.  Sums and scales are 32-bit, and so is the product of a block's two scales
+    (below 2^-126 it loses digits); the result is rounded once to
     ``out_dtype`` (float32 or bfloat16; default: that of ``out``, or x's, or bfloat16 where x is in 8 bits)."""
     values = weight.values
     if values.dim() != 2 or not _sound(weight, BLOCK):

@@ -25,7 +25,7 @@ from ..weights.declare import WeightDecl
 
 @dataclass
 class Runtime:
-    """``products``: in what the matrices of dense SiLU-gated feed-forwards and of the output head are held; "same" (the dtype) or
+    """``products``: in what the matrices of ``swiglu`` feed-forwards and of the output head are held; "same" (the dtype, as all other matrices) or
     "float8" (8 bits with a scale for each 128 x 128, their inputs brought to 8 bits row by row)."""
     dtype: torch.dtype
     device: torch.device
